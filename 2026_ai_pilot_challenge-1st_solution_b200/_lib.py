@@ -4,6 +4,7 @@ The library is built in-tree by ``build.py``.  There is no fallback: if the libr
 missing or cannot be loaded, importing the GPU entry points raises, so a GPU run can never
 silently take a CPU path.
 """
+import contextlib
 import ctypes as C
 from pathlib import Path
 
@@ -63,6 +64,31 @@ class PayoffArgs(C.Structure):
                 ("final_step", C.c_void_p), ("nonfinite", C.c_void_p), ("step_dev", C.c_void_p)]
 
 
+class ScanArgs(C.Structure):
+    """f16_scan_args (include/f16env.h)."""
+    _fields_ = [("dtype", C.c_int), ("gated", C.c_int), ("steps", C.c_int64), ("batch", C.c_int64),
+                ("dim", C.c_int64), ("gate", C.c_void_p), ("gate_t", C.c_int64), ("gate_b", C.c_int64),
+                ("x", C.c_void_p), ("x_t", C.c_int64), ("x_b", C.c_int64), ("h0", C.c_void_p),
+                ("reset", C.c_void_p), ("reset_bytes", C.c_int), ("reset_t", C.c_int64), ("reset_b", C.c_int64),
+                ("lengths", C.c_void_p), ("h", C.c_void_p), ("h_t", C.c_int64), ("h_b", C.c_int64),
+                ("hn", C.c_void_p), ("saved", C.c_void_p), ("dh", C.c_void_p), ("dh_t", C.c_int64),
+                ("dh_b", C.c_int64), ("dhn", C.c_void_p), ("dgate", C.c_void_p), ("dgate_t", C.c_int64),
+                ("dgate_b", C.c_int64), ("dx", C.c_void_p), ("dx_t", C.c_int64), ("dx_b", C.c_int64),
+                ("dh0", C.c_void_p)]
+
+
+class AdamwArgs(C.Structure):
+    """f16_adamw_args (include/f16env.h)."""
+    _fields_ = [("count", C.c_int), ("dtype", C.c_int), ("state_bits", C.c_int), ("params_host", C.c_void_p),
+                ("grads_host", C.c_void_p), ("numel_host", C.c_void_p), ("first_host", C.c_void_p),
+                ("index_host", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("weight_decay", C.c_double), ("max_norm", C.c_double),
+                ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exp_avg_scale", C.c_void_p),
+                ("exp_avg_sq_scale", C.c_void_p), ("master", C.c_void_p), ("steps", C.c_void_p),
+                ("ticket", C.c_void_p), ("partial", C.c_void_p), ("partials", C.c_int), ("norm", C.c_void_p),
+                ("seed", C.c_uint64)]
+
+
 _PR = C.POINTER(Recon)
 _PC = C.POINTER(RewardCfg)
 _PO = C.POINTER(Origin)
@@ -109,6 +135,18 @@ _SIGS = {
                                  C.c_int),
     "f16_categorical_fwd": ([_P, _I64, _I64, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _P], C.c_int),
     "f16_categorical_bwd": ([_P, _I64, _I64, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _I64, _P], C.c_int),
+    "f16_layer_norm_fwd": ([_P, _I64, C.c_int, _I64, C.c_int, _P, _P, C.c_int, C.c_double, _P, _I64, _P, _P, _P],
+                           C.c_int),
+    "f16_layer_norm_bwd": ([_P, _I64, _P, _I64, _I64, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _I64, _P, _P, _P,
+                            _I64, _P], C.c_int),
+    "f16_layer_norm_scratch_floats": ([_I64, C.c_int], _I64),
+    "f16_scan_saved_floats": ([_I64, _I64, _I64], _I64),
+    "f16_scan_fwd": ([C.POINTER(ScanArgs), _P], C.c_int),
+    "f16_scan_bwd": ([C.POINTER(ScanArgs), _P], C.c_int),
+    "f16_scan_step": ([_P, _I64, _P, _I64, _I64, _I64, C.c_int, C.c_int, _P, C.c_int, _I64, _P, _I64, _P, _I64, _P],
+                      C.c_int),
+    "f16_grad_squares": ([C.c_int, _P, _P, C.c_int, _P, C.c_int, C.POINTER(C.c_int), _P], C.c_int),
+    "f16_adamw_step": ([C.POINTER(AdamwArgs), _P], C.c_int),
     "f16_seed_ic": ([_P, _I64, _P, C.c_int, _I64, C.c_double, _P], C.c_int),
     "f16_probe_fp64": ([_P, _I64, C.c_int, C.POINTER(C.c_double), _P], C.c_int),
     "f16_version": ([], C.c_char_p),
@@ -152,6 +190,16 @@ def ptr(t):
 def stream_of(t):
     """Raw handle of the torch current stream on the tensor's device."""
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+# dtype codes of the training operators (F16_DTYPE_* in include/f16env.h)
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Context in which the tensor's device is the current one (launches go to the current device)."""
+    return _SAME_DEVICE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def require_cuda_tensor(t, dtype, shape, label, device=None):

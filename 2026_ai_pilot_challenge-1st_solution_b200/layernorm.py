@@ -1,0 +1,107 @@
+"""Layer norm over the last axis on the sm_100a kernels, with its gradient.
+
+``layer_norm(x, weight, bias, eps)`` is ``torch.nn.functional.layer_norm`` over the last axis for CUDA
+tensors: fp32, bf16 or fp16 input, weight and bias in fp32 or the input's type (either may be
+None), statistics and sums in fp32, one rounding when a value is stored.  Backward gives the
+gradients of x, weight and bias in two launches; the sums over rows behind the weight's and bias's
+are made in a fixed order, so the same inputs give the same bits.  ``LayerNorm`` is
+``torch.nn.LayerNorm`` over one axis with that forward (CPU tensors take torch's): a drop-in that
+keeps the parameter names, and that ``splitmm.run_tower`` takes between its layers.
+
+The reference normalises observations only (``rollout.RunningNorm``) and has no counterpart.
+"""
+import torch
+
+from . import _lib
+
+
+def _rows(x):
+    """x as (rows, dim) with unit column stride (a view where its layout allows)."""
+    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    return x if x.stride(1) == 1 and x.stride(0) >= 0 or x.shape[1] == 1 else x.contiguous()
+
+
+def _row_stride(x):
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        rows = _rows(x)
+        n, dim = rows.shape
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = None
+        if any(ctx.needs_input_grad):
+            stats = torch.empty(2, n, dtype=torch.float32, device=x.device)
+        wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+        if weight is not None:
+            weight = weight.contiguous()
+        if bias is not None:
+            bias = bias.contiguous()
+        if n:
+            with _lib.on_device(x):
+                _lib.check(_lib.load().f16_layer_norm_fwd(
+                    rows.data_ptr(), n, dim, _row_stride(rows), _lib.DTYPES[x.dtype], _lib.ptr(weight),
+                    _lib.ptr(bias), _lib.DTYPES[wdtype], eps, y.data_ptr(), dim,
+                    stats.data_ptr() if stats is not None else None,
+                    stats.data_ptr() + 4 * n if stats is not None else None, _lib.stream_of(x)), "f16_layer_norm_fwd")
+        ctx.wdtype = wdtype
+        ctx.save_for_backward(rows, weight, stats)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        n, dim = x.shape
+        shape = dy.shape
+        dy = _rows(dy)
+        dx = torch.empty(shape, dtype=x.dtype, device=x.device) if need_x else None
+        if not n:
+            zero = torch.zeros(dim, dtype=ctx.wdtype, device=x.device) if need_w or need_b else None
+            return dx, zero if need_w else None, zero.clone() if need_b else None, None
+        dw = torch.empty(dim, dtype=ctx.wdtype, device=x.device) if need_w else None
+        db = torch.empty(dim, dtype=ctx.wdtype, device=x.device) if need_b else None
+        lib = _lib.load()
+        with _lib.on_device(x):
+            room = int(lib.f16_layer_norm_scratch_floats(n, dim)) if need_w or need_b else 0
+            scratch = torch.empty(room, dtype=torch.float32, device=x.device) if room else None
+            _lib.check(lib.f16_layer_norm_bwd(
+                dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), n, dim, _lib.DTYPES[x.dtype],
+                _lib.ptr(weight), _lib.DTYPES[ctx.wdtype], stats.data_ptr(), stats.data_ptr() + 4 * n, _lib.ptr(dx), dim,
+                _lib.ptr(dw), _lib.ptr(db), _lib.ptr(scratch), room, _lib.stream_of(x)), "f16_layer_norm_bwd")
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (module docstring)."""
+    _lib.require_cuda_tensor(x, tuple(_lib.DTYPES), None, "layer_norm input")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layer_norm needs a last axis of at least one value")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    dim = x.shape[-1]
+    for t, name in ((weight, "layer_norm weight"), (bias, "layer_norm bias")):
+        if t is not None:
+            _lib.require_cuda_tensor(t, (torch.float32, x.dtype), (dim,), name, x.device)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError("layer_norm weight and bias must have the same dtype")
+    return _LayerNorm.apply(x, weight, bias, float(eps))
+
+
+class LayerNorm(torch.nn.LayerNorm):
+    """torch.nn.LayerNorm over the last axis; CUDA tensors run through ``layer_norm``."""
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=None):
+        super().__init__(normalized_shape, eps, elementwise_affine, bias, device, dtype)
+        if len(self.normalized_shape) != 1:
+            raise ValueError("LayerNorm normalises the last axis only")
+
+    def forward(self, x):
+        if not x.is_cuda:
+            return super().forward(x)
+        if x.shape[-1:] != torch.Size(self.normalized_shape):
+            raise ValueError(f"input's last axis {tuple(x.shape[-1:])} != {tuple(self.normalized_shape)}")
+        return layer_norm(x, self.weight, self.bias, self.eps)

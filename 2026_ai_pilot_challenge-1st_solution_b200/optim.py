@@ -1,0 +1,230 @@
+"""AdamW over many tensors in one launch, the gradients' clip included, moments in 32 or 8 bits.
+
+``AdamW`` is ``torch.optim.AdamW`` (decoupled weight decay; with ``weight_decay=0`` torch.optim.Adam,
+the reference's optimiser, R/cuda_fdm/ppo_gpu.py:1300) for CUDA parameters, as a
+``torch.optim.Optimizer``: groups, schedulers, ``state_dict`` as usual.  What it adds:
+
+* ``max_grad_norm`` scales the gradients as ``torch.nn.utils.clip_grad_norm_`` over all parameters
+  does, without a pass that rewrites them; ``grad_norm`` is the norm of the last step, on the device.
+* ``state_bits=8`` keeps exp_avg as e4m3 and exp_avg_sq as e5m2 with a fp32 scale for every 256
+  values: 2 bytes a parameter in place of 8.  The codes are rounded stochastically (a hash of seed, step
+  and position): a moment moves by far less than a code's step at a time, rounded to nearest it would
+  stay where it is.
+* ``master_weights`` (16-bit parameters): fp32 copies that are updated and rounded into the
+  parameters, without which an update below half a step of the parameter is lost.  A parameter that was set
+  from outside since (a loaded checkpoint) is taken as it is.
+* Step counts live on the device: a step captured into a CUDA graph counts on every replay.  The
+  learning rate and the other numbers are those of the capture.
+
+Moments, masters and step counts of a group's tensors of one type lie in flat buffers
+(``state_buffers``); ``state[p]`` holds the tensors' views of them.
+"""
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+BLOCK = 256                     # F16_ADAMW_BLOCK: values that share a scale
+LAUNCH_TENSORS, LAUNCH_PARTIALS = 720, 592      # tensors of one launch, and the partial sums it may write
+
+
+class _Bucket:
+    """The tensors of one type in a parameter group, and their state in flat buffers."""
+
+    def __init__(self, params, bits, master):
+        self.params = params
+        self.dtype, self.device = params[0].dtype, params[0].device
+        self.firsts, total = [], 0
+        for p in params:
+            self.firsts.append(total)
+            total += -(-p.numel() // BLOCK) * BLOCK
+        zeros = lambda n, dtype: torch.zeros(n, dtype=dtype, device=self.device)
+        self.buffers = {}
+        if bits == 8:
+            self.buffers["exp_avg"] = zeros(total, torch.float8_e4m3fn)
+            self.buffers["exp_avg_scale"] = zeros(total // BLOCK, torch.float32)
+            self.buffers["exp_avg_sq"] = zeros(total, torch.float8_e5m2)
+            self.buffers["exp_avg_sq_scale"] = zeros(total // BLOCK, torch.float32)
+        else:
+            self.buffers["exp_avg"] = zeros(total, torch.float32)
+            self.buffers["exp_avg_sq"] = zeros(total, torch.float32)
+        if master:
+            self.buffers["master"] = zeros(total, torch.float32)
+        self.buffers["step"] = zeros(len(params), torch.int64)
+        self.ticket = zeros(1, torch.int32)
+
+    def views(self, i):
+        """The state of tensor i: views of the flat buffers."""
+        n, first = self.params[i].numel(), self.firsts[i]
+        out = {}
+        for name, flat in self.buffers.items():
+            if name == "step":
+                out[name] = flat[i]
+            elif name.endswith("_scale"):
+                out[name] = flat[first // BLOCK:first // BLOCK - (-n // BLOCK)]
+            else:
+                out[name] = flat[first:first + n].view(self.params[i].shape)
+        return out
+
+    def arguments(self, bits):
+        """(AdamwArgs with the table of the tensors that have a gradient, what it points to), or None."""
+        live = [i for i, p in enumerate(self.params) if p.grad is not None and p.numel()]
+        if not live:
+            return None
+        n = len(live)
+        params, grads, keep = [], [], []
+        for i in live:
+            p, g = self.params[i], self.params[i].grad
+            if g.is_sparse:
+                raise RuntimeError("AdamW does not take sparse gradients")
+            if p.dtype != self.dtype or p.device != self.device or not p.is_contiguous():
+                raise RuntimeError("a parameter's type, device or layout changed after the optimiser was made")
+            if g.dtype != self.dtype or g.device != self.device:
+                raise TypeError(f"a gradient must be {self.dtype} on {self.device} as its parameter is")
+            if not g.is_contiguous():
+                g = g.contiguous()
+            keep.append(g)
+            params.append(p.data_ptr())
+            grads.append(g.data_ptr())
+        a = _lib.AdamwArgs()
+        arrays = ((C.c_void_p * n)(*params), (C.c_void_p * n)(*grads),
+                  (C.c_int64 * n)(*[self.params[i].numel() for i in live]),
+                  (C.c_int64 * n)(*[self.firsts[i] for i in live]), (C.c_int32 * n)(*live))
+        a.count, a.dtype, a.state_bits = n, _lib.DTYPES[self.dtype], bits
+        a.params_host, a.grads_host, a.numel_host, a.first_host, a.index_host = (C.addressof(x) for x in arrays)
+        b = self.buffers
+        a.exp_avg, a.exp_avg_sq = b["exp_avg"].data_ptr(), b["exp_avg_sq"].data_ptr()
+        if bits == 8:
+            a.exp_avg_scale, a.exp_avg_sq_scale = b["exp_avg_scale"].data_ptr(), b["exp_avg_sq_scale"].data_ptr()
+        if "master" in b:
+            a.master = b["master"].data_ptr()
+        a.steps, a.ticket = b["step"].data_ptr(), self.ticket.data_ptr()
+        return a, (arrays, keep, [self.params[i] for i in live])
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW on the sm_100a kernels (module docstring).
+
+    state_bits       32 or 8, of exp_avg and exp_avg_sq
+    max_grad_norm    limit of the gradients' norm over all groups, or None
+    master_weights   fp32 copies of bf16 / fp16 parameters
+    seed             of the 8-bit moments' rounding
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32,
+                 max_grad_norm=None, master_weights=True, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError("max_grad_norm must be above 0, or None")
+        self.state_bits, self.master_weights = int(state_bits), bool(master_weights)
+        self.max_grad_norm, self.seed = max_grad_norm, int(seed) & (2 ** 64 - 1)
+        self.grad_norm = None
+        self._buckets = []          # one list of _Bucket for each group
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    @staticmethod
+    def _check_numbers(group):
+        lr, (b1, b2) = group["lr"], group["betas"]
+        if isinstance(lr, torch.Tensor):
+            raise TypeError("lr must be a number")
+        if not (lr >= 0.0 and group["eps"] >= 0.0 and group["weight_decay"] >= 0.0):
+            raise ValueError("lr, eps and weight_decay must not be negative")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError("betas must lie in [0, 1)")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            self._check_numbers(group)
+            kinds, seen = {}, set()
+            for p in group["params"]:
+                _lib.require_cuda_tensor(p, tuple(_lib.DTYPES), None, "AdamW parameter")
+                if not p.is_contiguous():
+                    raise ValueError("AdamW parameters must be contiguous")
+                if id(p) in seen:
+                    raise ValueError("a parameter appears twice in the group")
+                seen.add(id(p))
+                kinds.setdefault((p.dtype, p.device), []).append(p)
+            if len({d for _, d in kinds} | {b.device for bs in self._buckets for b in bs}) > 1:
+                raise ValueError("AdamW parameters must lie on one device")
+        except Exception:
+            self.param_groups.pop()
+            raise
+        buckets = [_Bucket(ps, self.state_bits, self.master_weights and dtype != torch.float32)
+                   for (dtype, _), ps in kinds.items()]
+        self._buckets.append(buckets)
+        for b in buckets:
+            for i, p in enumerate(b.params):
+                self.state[p] = b.views(i)
+
+    def state_buffers(self):
+        """The flat buffers behind the state, one dict for each group and parameter type: "exp_avg",
+        "exp_avg_sq" (with "_scale" each for 8-bit states), "master" where there are masters, "step".
+        A tensor begins at a multiple of 256 values, in the order of the group's parameters."""
+        return [b.buffers for bs in self._buckets for b in bs]
+
+    def load_state_dict(self, state_dict):
+        """Copies a state of the same form (state_bits, masters, shapes) into the flat buffers."""
+        groups = state_dict["param_groups"]
+        if len(groups) != len(self.param_groups) or any(
+                len(g["params"]) != len(h["params"]) for g, h in zip(groups, self.param_groups)):
+            raise ValueError("the state's parameter groups differ from the optimiser's")
+        pairs = [(k, p) for g, h in zip(groups, self.param_groups) for k, p in zip(g["params"], h["params"])]
+        for k, p in pairs:
+            new, old = state_dict["state"].get(k), self.state[p]
+            if new is not None and (new.keys() != old.keys() or any(
+                    tuple(new[n].shape) != tuple(old[n].shape) or new[n].dtype != old[n].dtype for n in old)):
+                raise ValueError("a tensor's state differs in form (state_bits, master_weights or shape)")
+        for g, h in zip(groups, self.param_groups):
+            self._check_numbers({**h, **{k: v for k, v in g.items() if k != "params"}})
+        for g, h in zip(groups, self.param_groups):
+            h.update({k: v for k, v in g.items() if k != "params"})
+        for k, p in pairs:
+            new = state_dict["state"].get(k)
+            for n, t in self.state[p].items():
+                t.zero_() if new is None else t.copy_(new[n])
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step over every parameter with a gradient; returns the closure's loss, if any."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls = []
+        for group, buckets in zip(self.param_groups, self._buckets):
+            self._check_numbers(group)
+            for b in buckets:
+                made = b.arguments(self.state_bits)
+                if made is not None:
+                    calls.append((group, b, *made))
+        if not calls:
+            return loss
+        lib = _lib.load()
+        device = calls[0][1].buffers["step"]
+        with _lib.on_device(device):
+            stream = _lib.stream_of(device)
+            partial, used = None, 0
+            if self.max_grad_norm is not None:
+                room = sum(-(-a.count // LAUNCH_TENSORS) for _, _, a, _ in calls) * LAUNCH_PARTIALS
+                partial = torch.empty(room, dtype=torch.float64, device=device.device)
+                self.grad_norm = torch.empty((), dtype=torch.float32, device=device.device)
+                for _, _, a, _ in calls:
+                    n = C.c_int(0)
+                    _lib.check(lib.f16_grad_squares(a.count, a.grads_host, a.numel_host, a.dtype,
+                                                    partial.data_ptr() + 8 * used, room - used, C.byref(n), stream),
+                               "f16_grad_squares")
+                    used += n.value
+            for group, _, a, (_, _, params) in calls:
+                a.lr, a.eps, a.weight_decay = float(group["lr"]), float(group["eps"]), float(group["weight_decay"])
+                a.beta1, a.beta2 = group["betas"]
+                if partial is not None:
+                    a.max_norm, a.partial, a.partials = float(self.max_grad_norm), partial.data_ptr(), used
+                    a.norm = self.grad_norm.data_ptr()
+                a.seed = self.seed
+                _lib.check(lib.f16_adamw_step(C.byref(a), stream), "f16_adamw_step")
+                torch.autograd.graph.increment_version(params)      # written behind autograd's back
+        return loss

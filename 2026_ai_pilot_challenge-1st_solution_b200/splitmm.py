@@ -36,6 +36,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from .layernorm import LayerNorm
 
 _BF = torch.bfloat16
 _F32 = torch.float32
@@ -316,8 +317,9 @@ def split_linear(x, weight, bias, act=ACT_NONE):
 
 
 def run_tower(seq, x):
-    """seq(x) for a Sequential of Linear and ReLU/Tanh modules: each Linear (+ the activation
-    that follows it) the split path takes runs as a SplitBlock, the others as plain fp32 torch."""
+    """seq(x) for a Sequential of Linear, ReLU/Tanh and ``layernorm.LayerNorm`` modules: each Linear
+    (+ the activation that follows it) the split path takes runs as a SplitBlock, a LayerNorm through
+    its kernels, the others as plain fp32 torch."""
     mods = list(seq)
     xs = None
     i = 0
@@ -327,7 +329,7 @@ def run_tower(seq, x):
             x, xs = m(x), None
             i += 1
             continue
-        act_mod = mods[i + 1] if i + 1 < len(mods) and not isinstance(mods[i + 1], nn.Linear) else None
+        act_mod = mods[i + 1] if i + 1 < len(mods) and not isinstance(mods[i + 1], (nn.Linear, LayerNorm)) else None
         code = ACT_NONE if act_mod is None else _ACT_CODES.get(type(act_mod))
         if code is None or not usable(m, x):
             x, xs = F.linear(x, m.weight, m.bias), None

@@ -35,6 +35,7 @@ import torch.nn as nn
 from . import _lib
 from . import categorical
 from . import splitmm
+from .optim import AdamW
 from .policy import HEAD_CATEGORICAL, HEAD_VALUE, MlpWeights, PolicySet
 from .rollout import RunningNorm, cast_half, gae, half_operand, make_action_grid
 
@@ -144,6 +145,31 @@ class PPOConfig:
     # 16-bit operand type of the rollout-time policy kernel: "fp16" keeps logits / log-probs
     # within 1e-3 of the fp32 networks at the same tensor rate as "bf16" (about 4e-3)
     policy_operand: str = "fp16"
+    # "adam": torch.optim.Adam after clip_grad_norm_, as the reference; "adamw": optim.AdamW, the clip
+    # inside its step, with `weight_decay` and moments of `state_bits` (32 or 8)
+    optimizer: str = "adam"
+    weight_decay: float = 0.0
+    state_bits: int = 32
+
+
+def make_optimizer(params, lr, cfg):
+    """The optimiser of a parameter list that ``cfg.optimizer`` names (eps 1e-5, ppo_gpu.py:1300)."""
+    if cfg.optimizer == "adam":
+        return torch.optim.Adam(params, lr=lr, eps=1e-5)
+    if cfg.optimizer == "adamw":
+        return AdamW(params, lr=lr, eps=1e-5, weight_decay=cfg.weight_decay, state_bits=cfg.state_bits,
+                     max_grad_norm=cfg.max_grad_norm, seed=cfg.seed)
+    raise ValueError("optimizer must be 'adam' or 'adamw'")
+
+
+def _clip_and_step(opt, params, max_norm):
+    """Clip the gradients of ``params`` to ``max_norm`` and step; returns their norm before the clip."""
+    if isinstance(opt, AdamW) and opt.max_grad_norm == max_norm:
+        opt.step()
+        return opt.grad_norm
+    norm = nn.utils.clip_grad_norm_(params, max_norm)
+    opt.step()
+    return norm
 
 
 class Opponent:
@@ -262,8 +288,7 @@ def _ppo_update(model, actor_opt, critic_opt, cfg, obs, act, old_logp, b_val, ad
             actor_loss = policy_loss - cfg.ent_coef * ent
             actor_loss.backward()
             _allreduce_mean_(model.actor_parameters(), group, world)
-            last_actor_grad = nn.utils.clip_grad_norm_(model.actor_parameters(), cfg.max_grad_norm)
-            actor_opt.step()
+            last_actor_grad = _clip_and_step(actor_opt, model.actor_parameters(), cfg.max_grad_norm)
 
             new_value = model.get_value(mb_obs)
             value_loss = 0.5 * ((new_value - returns.index_select(0, mb)) ** 2).mean()
@@ -271,8 +296,7 @@ def _ppo_update(model, actor_opt, critic_opt, cfg, obs, act, old_logp, b_val, ad
             critic_loss = cfg.vf_coef * value_loss
             critic_loss.backward()
             _allreduce_mean_(model.critic_parameters(), group, world)
-            last_critic_grad = nn.utils.clip_grad_norm_(model.critic_parameters(), cfg.max_grad_norm)
-            critic_opt.step()
+            last_critic_grad = _clip_and_step(critic_opt, model.critic_parameters(), cfg.max_grad_norm)
             optimizer_steps += 1
 
             with torch.no_grad():
@@ -331,8 +355,8 @@ class PPOTrainer:
                                group=group)
         self.norm = RunningNorm(OBS_DIM, dev) if cfg.normalize_obs else None
         clr = cfg.lr if cfg.critic_lr is None else cfg.critic_lr
-        self.actor_opt = torch.optim.Adam(self.model.actor_parameters(), lr=cfg.lr, eps=1e-5)
-        self.critic_opt = torch.optim.Adam(self.model.critic_parameters(), lr=clr, eps=1e-5)
+        self.actor_opt = make_optimizer(self.model.actor_parameters(), cfg.lr, cfg)
+        self.critic_opt = make_optimizer(self.model.critic_parameters(), clr, cfg)
         self.grid = make_action_grid(cfg.num_bins, device=dev)
         if not keep_terminal_obs:
             env.terminal_obs_enabled = False      # collect_rollout never reads info["terminal_obs"]

@@ -513,6 +513,124 @@ int f16_categorical_bwd(const float* logits, int64_t ldz, int64_t M, int A, int 
                         f16_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Training operators (no counterpart in the reference, whose networks are plain MLPs trained by
+ * torch.optim.Adam, R/cuda_fdm/ppo_gpu.py:1300): layer norm, a gated linear recurrence over
+ * time, AdamW over many tensors.  Values of dtype bf16 / fp16 / fp32 are computed with in fp32 and
+ * rounded to nearest once, when stored.
+ * ---------------------------------------------------------------------------------------- */
+#define F16_DTYPE_BF16 0
+#define F16_DTYPE_FP16 1
+#define F16_DTYPE_FP32 2
+
+/* Layer norm of x [rows][cols] (row stride ldx, 0 allowed) over a row:
+ * y = (x - mu) r w + b, mu the row's mean, r = 1 / sqrt(mean((x - mu)^2) + eps); weight / bias [cols]
+ * of type wdtype or NULL (1 / 0).  mean / rstd [rows]: the statistics the backward pass reads (both
+ * or neither).  Pointers are aligned to their type; 16-byte aligned rows run fastest. */
+int f16_layer_norm_fwd(const void* x, int64_t rows, int cols, int64_t ldx, int dtype, const void* weight,
+                       const void* bias, int wdtype, double eps, void* y, int64_t ldy, float* mean,
+                       float* rstd, f16_stream_t stream);
+
+/* Its gradient, with xh = (x - mu) r, g = dy w: dx = r (g - mean(g) - xh mean(g xh)),
+ * dweight = sum over rows of dy xh, dbias = sum over rows of dy (type wdtype), each NULL where it is
+ * not wanted.  scratch (at least 2 cols floats, f16_layer_norm_scratch_floats for full speed) is
+ * needed where dweight or dbias is: the sums are made in a fixed order. */
+int f16_layer_norm_bwd(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t rows, int cols,
+                       int dtype, const void* weight, int wdtype, const float* mean, const float* rstd,
+                       void* dx, int64_t ldd, void* dweight, void* dbias, float* scratch,
+                       int64_t scratch_floats, f16_stream_t stream);
+int64_t f16_layer_norm_scratch_floats(int64_t rows, int cols);
+
+/* A gated linear recurrence over time, each of batch x dim channels by itself:
+ *   gated 0: h_t = gate_t h_{t-1} + x_t;   gated 1: f = sigmoid(gate_t), h_t = f h_{t-1} + (1 - f) x_t,
+ * from h_{-1} = h0.  A reset at (t, b) drops the state before (h_t = x_t, or (1 - f) x_t); steps from
+ * lengths[b] on (clamped to 0..steps) leave the state as it is, write h_t = 0 and are not read.  hn is
+ * the state after the last step.  Element (t, b, d) of a sequence tensor lies at
+ * t stride_t + b stride_b + d (strides in elements, any sign or 0 where it is only read); states are
+ * [batch][dim] fp32, contiguous.  16-bit tensors whose rows are 4-byte aligned and even run faster.
+ * The forward pass writes `saved` (f16_scan_saved_floats values, or NULL where no gradient follows): the
+ * state before every F16_SCAN_CHUNK steps.  The backward pass reads it with gate, x and the gradients
+ * dh and dhn (one of them may be NULL: zero) and writes dgate, dx and dh0, each NULL where not
+ * wanted.  Coefficients above 1 in size: the product of any F16_SCAN_CHUNK x 16 successive ones has
+ * to stay in fp32's range. */
+#define F16_SCAN_CHUNK 16
+typedef struct {
+  int dtype;                   /* of gate, x, h and their gradients */
+  int gated;
+  int64_t steps, batch, dim;
+  const void* gate;
+  int64_t gate_t, gate_b;
+  const void* x;
+  int64_t x_t, x_b;
+  const float* h0;             /* or NULL: zero */
+  const void* reset;           /* [steps][batch] flags, nonzero: reset; or NULL */
+  int reset_bytes;             /* 1 (uint8) or 4 (fp32) */
+  int64_t reset_t, reset_b;
+  const int64_t* lengths;      /* [batch] or NULL */
+  void* h;
+  int64_t h_t, h_b;
+  float* hn;                   /* or NULL */
+  float* saved;
+  const void* dh;
+  int64_t dh_t, dh_b;
+  const float* dhn;
+  void* dgate;
+  int64_t dgate_t, dgate_b;
+  void* dx;
+  int64_t dx_t, dx_b;
+  float* dh0;
+} f16_scan_args;
+int64_t f16_scan_saved_floats(int64_t steps, int64_t batch, int64_t dim);
+int f16_scan_fwd(const f16_scan_args* args, f16_stream_t stream);
+int f16_scan_bwd(const f16_scan_args* args, f16_stream_t stream);
+
+/* One step of it (a decision): state [batch][dim] fp32 (row stride state_b) updated in place and
+ * written to h [batch][dim] in dtype; reset [batch] (element stride reset_b) or NULL. */
+int f16_scan_step(const void* gate, int64_t gate_b, const void* x, int64_t x_b, int64_t batch, int64_t dim,
+                  int dtype, int gated, const void* reset, int reset_bytes, int64_t reset_b, float* state,
+                  int64_t state_b, void* h, int64_t h_b, f16_stream_t stream);
+
+/* Squares of the gradients of `count` tensors of one dtype (grads_host / numel_host: host arrays of
+ * device pointers and element counts, read before the call returns), summed into fp64 partial sums
+ * partial[0..*used_host) in a fixed order; room: the values `partial` holds (592 for each 720 tensors
+ * keep every SM busy, 1 for each 720 is the least). */
+int f16_grad_squares(int count, const void* const* grads_host, const int64_t* numel_host, int dtype,
+                     double* partial, int room, int* used_host, f16_stream_t stream);
+
+/* One AdamW step over `count` tensors (torch.optim.AdamW's formulas, after
+ * torch.nn.utils.clip_grad_norm_'s scaling by min(1, max_norm / (norm + 1e-6)) where partial is given:
+ * norm^2 is the sum of its `partials` values; the gradients themselves stay as they are).  Moments,
+ * masters and step counts lie in flat device buffers: tensor i's values begin at first_host[i], a
+ * multiple of F16_ADAMW_BLOCK, and the tail of its last block belongs to it; its step count is
+ * steps[index_host[i]], raised on the device.  state_bits 32: fp32 moments.  8: exp_avg e4m3,
+ * exp_avg_sq e5m2, in units of a fp32 scale for each F16_ADAMW_BLOCK values, rounded stochastically by a
+ * hash of (seed, step, position).  master: fp32 copies of 16-bit parameters or NULL.  *ticket is zero
+ * before the first call and between calls.  One tensor may not appear twice. */
+#define F16_ADAMW_BLOCK 256
+typedef struct {
+  int count;
+  int dtype;                        /* of parameters and gradients */
+  int state_bits;
+  void* const* params_host;
+  const void* const* grads_host;
+  const int64_t* numel_host;
+  const int64_t* first_host;
+  const int32_t* index_host;
+  double lr, beta1, beta2, eps, weight_decay, max_norm;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* master;
+  int64_t* steps;
+  uint32_t* ticket;
+  const double* partial;            /* or NULL: no clipping */
+  int partials;
+  float* norm;                      /* or NULL; written where partial is given */
+  uint64_t seed;
+} f16_adamw_args;
+int f16_adamw_step(const f16_adamw_args* args, f16_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference): FP64 FMA-pipe probe, the measured roofline
  * denominator of the FDM kernel.  Launches `blocks` x 256 threads running 8 independent FMA
  * chains for `iters` iterations; *flops receives the FP64 flop count (host pointer).
