@@ -27,6 +27,7 @@
 // selection (never a product with 0), so that an infinity or NaN left by the episode before does not
 // leak: a coefficient that is NaN itself makes B NaN as well, so the two cannot be confused.
 #include <cooperative_groups.h>
+#include <type_traits>
 #include "typed.cuh"
 
 namespace cg = cooperative_groups;
@@ -38,26 +39,40 @@ constexpr int CHUNK = F16_SCAN_CHUNK;     // steps in registers at a time, betwe
 constexpr int MAX_WARPS = 16;             // of a block on consecutive chunks
 constexpr int MAX_CLUSTER = 8;            // blocks of a cluster on consecutive chunks
 constexpr int WIDE_WARPS = 4;             // of a block whose warps have channels of their own
+constexpr int WIDE_BLOCKS = 5, WIDE_GRAD_BLOCKS = 3;      // of those on an SM: 96 and 168 registers a thread
 static_assert(CHUNK <= 32, "resets of a chunk are bits of one word");
 
 typedef f16_scan_args Args;
 
-// Sigmoid and its complement without cancellation: e = exp(-|g|), the larger is 1 / (1 + e).
-__device__ __forceinline__ void gates(float g, float& f, float& k) {
-  const float e = __expf(-fabsf(g)), big = __fdividef(1.0f, 1.0f + e), small = e * big;
-  f = g >= 0.0f ? big : small;
-  k = g >= 0.0f ? small : big;
-  if (g != g) f = k = g;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
+// A step's coefficients in one register.  Gated: the smaller one of f and 1 - f, e / (1 + e) with
+// e = exp(-|gate|), with the gate's sign: negative, it is f.  The other is its difference from 1, which
+// is at least 1/2 and so keeps every digit.  Raw: the coefficient itself.
 template <bool GATED>
-__device__ __forceinline__ void coefficients(float g, float x, float& a, float& b, float& k) {
+__device__ __forceinline__ float packed_gate(float g) {
+  if (!GATED) return g;
+  const float e = ex2(-1.4426950408889634f * fabsf(g));
+  return copysignf(e * rcp(1.0f + e), g);
+}
+template <bool GATED>
+__device__ __forceinline__ void coefficients(float s, float& a, float& k) {
   if (GATED) {
-    gates(g, a, k);
-    b = k * x;
+    const float small = fabsf(s), big = 1.0f - small;
+    const bool neg = __float_as_int(s) < 0;
+    a = neg ? small : big;
+    k = neg ? big : small;
   } else {
-    a = g;
-    b = x;
+    a = s;
     k = 1.0f;
   }
 }
@@ -70,15 +85,20 @@ __device__ __forceinline__ float pass_through(float A, float B, float h) {
 struct Lane {
   int64_t b, d, c;      // sequence, feature, channel = b dim + d
   bool live;            // the channel exists
+  bool together;        // all channels of the warp belong to one sequence
   int len;              // the sequence's steps
 };
 
+// Called by whole warps: c is the first of the lane's channels.
 __device__ __forceinline__ Lane lane_of(const Args& p, int64_t c) {
   Lane l;
   l.c = c;
   l.live = c < p.batch * p.dim;
   l.b = l.live ? c / p.dim : 0;
   l.d = l.live ? c - l.b * p.dim : 0;
+  const int64_t first = __shfl_sync(~0u, l.b, 0);
+  if (!l.live) l.b = first;
+  l.together = __all_sync(~0u, l.b == first);
   l.len = (int)p.steps;
   if (p.lengths) {
     const int64_t n = p.lengths[l.b];
@@ -87,33 +107,86 @@ __device__ __forceinline__ Lane lane_of(const Args& p, int64_t c) {
   return l;
 }
 
-// Bit i: step t0 + i resets the lane's sequence.
+__device__ __forceinline__ bool reset_at(const Args& p, int64_t b, int64_t t) {
+  const int64_t i = b * p.reset_b + t * p.reset_t;
+  return p.reset_bytes == 1 ? __ldg(reinterpret_cast<const uint8_t*>(p.reset) + i) != 0
+                            : __ldg(reinterpret_cast<const float*>(p.reset) + i) != 0.0f;
+}
+
+// Bit i: step t0 + i (of the n from t0 on) resets the lane's sequence.  Called by whole warps: where a warp
+// has one sequence its lanes read a step each.
 __device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0, int n) {
-  unsigned m = 0;
-  if (p.reset) {
-    if (p.reset_bytes == 1) {
-      const uint8_t* r = reinterpret_cast<const uint8_t*>(p.reset) + l.b * p.reset_b + (int64_t)t0 * p.reset_t;
-#pragma unroll
-      for (int i = 0; i < CHUNK; i++)
-        if (i < n) m |= (unsigned)(__ldg(r + (int64_t)i * p.reset_t) != 0) << i;
-    } else {
-      const float* r = reinterpret_cast<const float*>(p.reset) + l.b * p.reset_b + (int64_t)t0 * p.reset_t;
-#pragma unroll
-      for (int i = 0; i < CHUNK; i++)
-        if (i < n) m |= (unsigned)(__ldg(r + (int64_t)i * p.reset_t) != 0.0f) << i;
-    }
+  if (!p.reset) return 0;
+  if (l.together) {
+    const int lane = threadIdx.x & 31, m = l.len - t0 < CHUNK ? l.len - t0 : CHUNK;
+    return __ballot_sync(~0u, t0 >= 0 && lane < m && reset_at(p, l.b, t0 + lane));
   }
+  unsigned m = 0;
+#pragma unroll 1
+  for (int i = 0; i < n; i++) m |= (unsigned)reset_at(p, l.b, t0 + i) << i;
   return m;
 }
 
-// The first n of CHUNK steps from t0 on; the others are left alone.
 template <typename T, int V>
-__device__ __forceinline__ void load_chunk(Vec<T, V> (&v)[CHUNK], const void* base, int64_t st, int64_t sb, const Lane& l,
-                                           int t0, int n) {
-  const T* q = reinterpret_cast<const T*>(base) + l.b * sb + l.d + (int64_t)t0 * st;
+__device__ __forceinline__ void unpack(const Vec<T, V>& v, float (&f)[V]) {
+  if constexpr (sizeof(T) == 2 && V == 2) {
+    float2 two;
+    if constexpr (std::is_same<T, __half>::value) {
+      two = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    } else {
+      two = make_float2(__uint_as_float(v.r << 16), __uint_as_float(v.r & 0xffff0000u));
+    }
+    f[0] = two.x;
+    f[1] = two.y;
+  } else {
 #pragma unroll
-  for (int i = 0; i < CHUNK; i++)
-    if (i < n) v[i] = load_vec_nc<T, V>(q + (int64_t)i * st);
+    for (int k = 0; k < V; k++) f[k] = to_f32(v.e[k]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> pack(const float (&f)[V]) {
+  Vec<T, V> v;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && V == 2) {
+    const __nv_bfloat162 two = __floats2bfloat162_rn(f[0], f[1]);
+    v.r = *reinterpret_cast<const unsigned*>(&two);
+  } else if constexpr (std::is_same<T, __half>::value && V == 2) {
+    const __half2 two = __floats2half2_rn(f[0], f[1]);
+    v.r = *reinterpret_cast<const unsigned*>(&two);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) v.e[k] = from_f32<T>(f[k]);
+  }
+  return v;
+}
+
+// A tensor's element (t0, b, d), and how far it is to the next step's.
+template <typename T>
+struct Line {
+  T* p;
+  int64_t st;
+  __device__ __forceinline__ Line(const void* base, int64_t st, int64_t sb, const Lane& l, int t0)
+      : p(reinterpret_cast<T*>(const_cast<void*>(base)) + l.b * sb + l.d + (int64_t)t0 * st), st(st) {}
+};
+// One step on.  Opaque, so that a chunk's addresses are made one after the other and not all kept.
+template <typename T>
+__device__ __forceinline__ void advance(T*& q, int64_t by) {
+  q += by;
+  asm volatile("" : "+l"(q));
+}
+
+// The first n of CHUNK steps (ALL: every one); the others are left alone.
+template <typename T, int V, bool ALL>
+__device__ __forceinline__ void load_chunk(Vec<T, V> (&v)[CHUNK], Line<T> at, int n) {
+#pragma unroll
+  for (int i = 0; i < CHUNK; i++) {
+    if (ALL || i < n) v[i] = load_vec_nc<T, V>(at.p);
+    advance(at.p, at.st);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void load_chunk(Vec<T, V> (&v)[CHUNK], const Line<T>& at, int n, bool all) {
+  if (all) load_chunk<T, V, true>(v, at, n);
+  else load_chunk<T, V, false>(v, at, n);
 }
 
 template <int V>
@@ -185,8 +258,50 @@ __device__ __forceinline__ void join(Shared<V>& s, int half, int warps, int bloc
   }
 }
 
+// The steps of a chunk from the state h on, written to `out`.  PLAIN: every lane has all CHUNK steps and no
+// reset among them.  s: the packed coefficients (gated; raw ones are read from g).
+template <typename T, int V, bool GATED, bool PLAIN>
+__device__ __forceinline__ void walk(const Vec<T, V> (&g)[CHUNK], const float (&s)[GATED ? CHUNK : 1][V],
+                                     const Vec<T, V> (&x)[CHUNK], unsigned cut, int n, int left, bool live, Line<T> out,
+                                     float (&h)[V]) {
+#pragma unroll
+  for (int i = 0; i < CHUNK; i++) {
+    float xf[V], gf[V], o[V];
+    unpack<T, V>(x[i], xf);
+    if (!GATED) unpack<T, V>(g[i], gf);
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+      float a, c;
+      coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
+      const float b = GATED ? c * xf[k] : xf[k];
+      if (PLAIN) {
+        h[k] = fmaf(a, h[k], b);
+        o[k] = h[k];
+      } else {
+        if (i < n) h[k] = cut >> i & 1 ? b : fmaf(a, h[k], b);
+        o[k] = i < n ? h[k] : 0.0f;
+      }
+    }
+    if (PLAIN || (live && i < left)) store_vec<T, V>(out.p, pack<T, V>(o));
+    advance(out.p, out.st);
+  }
+}
+
+template <typename T, int V, bool GATED>
+__device__ __forceinline__ void pack_gates(const Vec<T, V> (&g)[CHUNK], float (&s)[GATED ? CHUNK : 1][V]) {
+  if constexpr (GATED) {
+#pragma unroll
+    for (int i = 0; i < CHUNK; i++) {
+      float gf[V];
+      unpack<T, V>(g[i], gf);
+#pragma unroll
+      for (int k = 0; k < V; k++) s[i][k] = packed_gate<true>(gf[k]);
+    }
+  }
+}
+
 template <typename T, int V, bool GATED, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS)
+__global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS, SPLIT ? 1 : WIDE_BLOCKS)
     k_scan(const __grid_constant__ Args p, int blocks) {
   const int warp = threadIdx.x >> 5, warps = SPLIT ? blockDim.x >> 5 : 1;
   const int rank = SPLIT ? (int)(blockIdx.x % blocks) : 0;
@@ -196,84 +311,127 @@ __global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS)
   float h[V];
   load_state<V>(h, p.h0, l);
   if (SPLIT && blocks > 1) cg::this_cluster().sync();      // every block has begun
+  const int mine = SPLIT ? (rank * warps + warp) * CHUNK : 0;
+  const auto steps_at = [&](int t0) { return l.live ? (l.len - t0 < CHUNK ? l.len - t0 : CHUNK) : 0; };
+  Vec<T, V> g[CHUNK], x[CHUNK];
+  const auto fetch = [&](int t0) {
+    const int n = steps_at(t0);
+    const bool all = __all_sync(~0u, n == CHUNK);
+    load_chunk<T, V>(g, Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
+    load_chunk<T, V>(x, Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
+    return resets_of(p, l, t0, n);
+  };
   int half = 0;
   for (int base = 0; base < T_; base += tile, half ^= 1) {
-    const int t0 = base + (SPLIT ? (rank * warps + warp) * CHUNK : 0);
-    const int left = T_ - t0, n = l.live ? (l.len - t0 < CHUNK ? l.len - t0 : CHUNK) : 0;
-    Vec<T, V> g[CHUNK], x[CHUNK];
-    load_chunk<T, V>(g, p.gate, p.gate_t, p.gate_b, l, t0, n);
-    load_chunk<T, V>(x, p.x, p.x_t, p.x_b, l, t0, n);
-    const unsigned cut = resets_of(p, l, t0, n);
+    const int t0 = base + mine, left = T_ - t0, n = steps_at(t0);
+    const unsigned cut = fetch(t0);
+    const bool plain = __all_sync(~0u, n == CHUNK && cut == 0);
+    float s[GATED ? CHUNK : 1][V];
+    pack_gates<T, V, GATED>(g, s);
+    float before[V];
     if (SPLIT) {
-      __shared__ Shared<V> s;
-      float A[V], B[V], before[V];
+      __shared__ Shared<V> sh;
+      float A[V], B[V];
 #pragma unroll
       for (int k = 0; k < V; k++) {
         A[k] = 1.0f;
         B[k] = 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < CHUNK; i++)
-        if (i < n) {
+      for (int i = 0; i < CHUNK; i++) {
+        float xf[V], gf[V];
+        unpack<T, V>(x[i], xf);
+        if (!GATED) unpack<T, V>(g[i], gf);
 #pragma unroll
-          for (int k = 0; k < V; k++) {
-            float a, b, c;
-            coefficients<GATED>(to_f32(g[i].e[k]), to_f32(x[i].e[k]), a, b, c);
-            if (cut >> i & 1) {
-              A[k] = __int_as_float(0x7fffffff);
-              B[k] = b;
-            } else {
-              A[k] *= a;
-              B[k] = fmaf(a, B[k], b);
-            }
+        for (int k = 0; k < V; k++) {
+          float a, c;
+          coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
+          const float b = GATED ? c * xf[k] : xf[k];
+          if (i < n) {
+            const bool r = cut >> i & 1;
+            A[k] = r ? __int_as_float(0x7fffffff) : A[k] * a;
+            B[k] = r ? b : fmaf(a, B[k], b);
           }
         }
-      join<V>(s, half, warps, blocks, rank, A, B, h, before);
+      }
+      join<V>(sh, half, warps, blocks, rank, A, B, h, before);
       // h is the state after the tile now; the chunk is repeated from `before`
-      if (p.saved && left > 0) store_state<V>(p.saved + (int64_t)(t0 / CHUNK) * p.batch * p.dim, before, l);
-      T* out = reinterpret_cast<T*>(p.h) + l.b * p.h_b + l.d + (int64_t)t0 * p.h_t;
-#pragma unroll
-      for (int i = 0; i < CHUNK; i++)
-        if (l.live && i < left) {
-          Vec<T, V> o;
-#pragma unroll
-          for (int k = 0; k < V; k++) {
-            if (i < n) {
-              float a, b, c;
-              coefficients<GATED>(to_f32(g[i].e[k]), to_f32(x[i].e[k]), a, b, c);
-              before[k] = cut >> i & 1 ? b : fmaf(a, before[k], b);
-            }
-            o.e[k] = from_f32<T>(i < n ? before[k] : 0.0f);
-          }
-          store_vec<T, V>(out + (int64_t)i * p.h_t, o);
-        }
     } else {
-      if (p.saved) store_state<V>(p.saved + (int64_t)(t0 / CHUNK) * p.batch * p.dim, h, l);
-      T* out = reinterpret_cast<T*>(p.h) + l.b * p.h_b + l.d + (int64_t)t0 * p.h_t;
 #pragma unroll
-      for (int i = 0; i < CHUNK; i++)
-        if (l.live && i < left) {
-          Vec<T, V> o;
+      for (int k = 0; k < V; k++) before[k] = h[k];
+    }
+    if (p.saved && left > 0) store_state<V>(p.saved + (int64_t)(t0 / CHUNK) * p.batch * p.dim, before, l);
+    const Line<T> out(p.h, p.h_t, p.h_b, l, t0);
+    if (plain) walk<T, V, GATED, true>(g, s, x, 0, CHUNK, CHUNK, true, out, before);
+    else walk<T, V, GATED, false>(g, s, x, cut, n, left, l.live, out, before);
+    if (!SPLIT) {
 #pragma unroll
-          for (int k = 0; k < V; k++) {
-            if (i < n) {
-              float a, b, c;
-              coefficients<GATED>(to_f32(g[i].e[k]), to_f32(x[i].e[k]), a, b, c);
-              h[k] = cut >> i & 1 ? b : fmaf(a, h[k], b);
-            }
-            o.e[k] = from_f32<T>(i < n ? h[k] : 0.0f);
-          }
-          store_vec<T, V>(out + (int64_t)i * p.h_t, o);
-        }
+      for (int k = 0; k < V; k++) h[k] = before[k];
     }
   }
   if (!SPLIT || (rank == 0 && warp == 0)) store_state<V>(p.hn, h, l);
 }
 
+// The steps of a chunk again from the saved state h, then their gradients from the last one back; carry: the
+// gradient that reaches the chunk's last state, then the one that leaves its first.
+// Gated: with d_t = f (h_{t-1} - x_t), dx_t = G k and dgate_t = dx_t d_t.
+template <typename T, int V, bool GATED, bool PLAIN>
+__device__ __forceinline__ void walk_back(const Vec<T, V> (&g)[CHUNK], const float (&s)[GATED ? CHUNK : 1][V],
+                                          const Vec<T, V> (&x)[CHUNK], const Vec<T, V> (&dh)[CHUNK], unsigned cut, int n,
+                                          int left, bool live, Line<T> dg, bool want_g, Line<T> dx, bool want_x,
+                                          float (&h)[V], float (&carry)[V]) {
+  float d[CHUNK][V];
+#pragma unroll
+  for (int i = 0; i < CHUNK; i++) {
+    float xf[V], gf[V];
+    unpack<T, V>(x[i], xf);
+    if (!GATED) unpack<T, V>(g[i], gf);
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+      float a, c;
+      coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
+      const float b = GATED ? c * xf[k] : xf[k];
+      const bool r = !PLAIN && (cut >> i & 1);
+      const float hp = r ? 0.0f : h[k];
+      d[i][k] = GATED ? a * (hp - xf[k]) : hp;
+      h[k] = r ? b : fmaf(a, hp, b);
+    }
+  }
+  const int last = CHUNK - 1;
+  dg.p += last * dg.st;
+  dx.p += last * dx.st;
+#pragma unroll
+  for (int i = CHUNK - 1; i >= 0; i--) {
+    float gf[V], df[V], og[V], ox[V];
+    unpack<T, V>(dh[i], df);
+    if (!GATED) unpack<T, V>(g[i], gf);
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+      float a, c;
+      coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
+      const float G = df[k] + carry[k];
+      ox[k] = GATED ? G * c : G;
+      og[k] = ox[k] * d[i][k];
+      if (PLAIN) {
+        carry[k] = a * G;
+      } else {
+        if (i < n) carry[k] = cut >> i & 1 ? 0.0f : a * G;
+        if (i >= n) og[k] = ox[k] = 0.0f;
+      }
+    }
+    if (PLAIN || (live && i < left)) {
+      if (want_g) store_vec<T, V>(dg.p, pack<T, V>(og));
+      if (want_x) store_vec<T, V>(dx.p, pack<T, V>(ox));
+    }
+    advance(dg.p, -dg.st);
+    advance(dx.p, -dx.st);
+  }
+}
+
 // Backward: tiles and chunks from the last to the first, the carried value the gradient of the state
 // before the steps already done.
 template <typename T, int V, bool GATED, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS)
+__global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS, SPLIT ? 1 : WIDE_GRAD_BLOCKS)
     k_scan_grad(const __grid_constant__ Args p, int blocks) {
   const int warp = threadIdx.x >> 5, warps = SPLIT ? blockDim.x >> 5 : 1;
   const int rank = SPLIT ? (int)(blockIdx.x % blocks) : 0;
@@ -288,22 +446,26 @@ __global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS)
     const int q = chunks - 1 - (done + (SPLIT ? rank * warps + warp : 0));      // below 0: nothing left
     const int t0 = q * CHUNK, left = q < 0 ? 0 : T_ - t0;
     const int n = l.live && q >= 0 ? (l.len - t0 < CHUNK ? l.len - t0 : CHUNK) : 0;
+    const bool all = __all_sync(~0u, n == CHUNK);
     Vec<T, V> g[CHUNK], x[CHUNK], dh[CHUNK];
-    load_chunk<T, V>(g, p.gate, p.gate_t, p.gate_b, l, t0, n);
-    load_chunk<T, V>(x, p.x, p.x_t, p.x_b, l, t0, n);
+    load_chunk<T, V>(g, Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
     if (p.dh) {
-      load_chunk<T, V>(dh, p.dh, p.dh_t, p.dh_b, l, t0, n);
+      load_chunk<T, V>(dh, Line<T>(p.dh, p.dh_t, p.dh_b, l, t0), n, all);
     } else {
 #pragma unroll
       for (int i = 0; i < CHUNK; i++)
 #pragma unroll
         for (int k = 0; k < V; k++) dh[i].e[k] = from_f32<T>(0.0f);
     }
+    load_chunk<T, V>(x, Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
     const unsigned cut = resets_of(p, l, t0, n);
-    float h[V], hp[CHUNK][V], c_in[V];
+    const bool plain = __all_sync(~0u, n == CHUNK && cut == 0);
+    float h[V], c_in[V];
     load_state<V>(h, n > 0 ? p.saved + (int64_t)q * p.batch * p.dim : nullptr, l);
+    float s[GATED ? CHUNK : 1][V];
+    pack_gates<T, V, GATED>(g, s);
     if (SPLIT) {
-      __shared__ Shared<V> s;
+      __shared__ Shared<V> sh;
       float A[V], B[V];
 #pragma unroll
       for (int k = 0; k < V; k++) {
@@ -311,62 +473,30 @@ __global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS)
         B[k] = 0.0f;
       }
 #pragma unroll
-      for (int i = CHUNK - 1; i >= 0; i--)
-        if (i < n) {
+      for (int i = CHUNK - 1; i >= 0; i--) {
+        float gf[V], df[V];
+        unpack<T, V>(dh[i], df);
+        if (!GATED) unpack<T, V>(g[i], gf);
 #pragma unroll
-          for (int k = 0; k < V; k++) {
-            float a, b, c;
-            coefficients<GATED>(to_f32(g[i].e[k]), 0.0f, a, b, c);
-            const float G = to_f32(dh[i].e[k]) + B[k];
-            if (cut >> i & 1) {
-              A[k] = __int_as_float(0x7fffffff);
-              B[k] = 0.0f;
-            } else {
-              A[k] *= a;
-              B[k] = a * G;
-            }
+        for (int k = 0; k < V; k++) {
+          float a, c;
+          coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
+          if (i < n) {
+            const bool r = cut >> i & 1;
+            A[k] = r ? __int_as_float(0x7fffffff) : A[k] * a;
+            B[k] = r ? 0.0f : a * (df[k] + B[k]);
           }
         }
-      join<V>(s, half, warps, blocks, rank, A, B, carry, c_in);
+      }
+      join<V>(sh, half, warps, blocks, rank, A, B, carry, c_in);
     } else {
 #pragma unroll
       for (int k = 0; k < V; k++) c_in[k] = carry[k];
     }
-#pragma unroll
-    for (int i = 0; i < CHUNK; i++)
-      if (i < n) {
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-          float a, b, c;
-          coefficients<GATED>(to_f32(g[i].e[k]), to_f32(x[i].e[k]), a, b, c);
-          hp[i][k] = cut >> i & 1 ? 0.0f : h[k];
-          h[k] = cut >> i & 1 ? b : fmaf(a, h[k], b);
-        }
-      }
-    T* dg = reinterpret_cast<T*>(p.dgate) + (p.dgate ? l.b * p.dgate_b + l.d + (int64_t)t0 * p.dgate_t : 0);
-    T* dx = reinterpret_cast<T*>(p.dx) + (p.dx ? l.b * p.dx_b + l.d + (int64_t)t0 * p.dx_t : 0);
-#pragma unroll
-    for (int i = CHUNK - 1; i >= 0; i--)
-      if (l.live && i < left) {
-        Vec<T, V> og, ox;
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-          float vg = 0.0f, vx = 0.0f;
-          if (i < n) {
-            float a, b, c;
-            const float xi = to_f32(x[i].e[k]);
-            coefficients<GATED>(to_f32(g[i].e[k]), xi, a, b, c);
-            const float G = to_f32(dh[i].e[k]) + c_in[k];
-            vg = GATED ? G * (hp[i][k] - xi) * (a * c) : G * hp[i][k];
-            vx = GATED ? G * c : G;
-            c_in[k] = cut >> i & 1 ? 0.0f : a * G;
-          }
-          og.e[k] = from_f32<T>(vg);
-          ox.e[k] = from_f32<T>(vx);
-        }
-        if (p.dgate) store_vec<T, V>(dg + (int64_t)i * p.dgate_t, og);
-        if (p.dx) store_vec<T, V>(dx + (int64_t)i * p.dx_t, ox);
-      }
+    const Line<T> dg(p.dgate, p.dgate_t, p.dgate_b, l, t0), dx(p.dx, p.dx_t, p.dx_b, l, t0);
+    const bool want_g = p.dgate, want_x = p.dx;
+    if (plain) walk_back<T, V, GATED, true>(g, s, x, dh, 0, CHUNK, CHUNK, true, dg, want_g, dx, want_x, h, c_in);
+    else walk_back<T, V, GATED, false>(g, s, x, dh, cut, n, left, l.live, dg, want_g, dx, want_x, h, c_in);
     if (!SPLIT) {
 #pragma unroll
       for (int k = 0; k < V; k++) carry[k] = c_in[k];
@@ -383,13 +513,13 @@ __global__ void __launch_bounds__(256)
                 int64_t state_b, T* __restrict__ out, int64_t out_b) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, per = dim / V;
   if (i >= batch * per) return;
-  const int64_t b = batch * per <= 0xffffffffll ? (unsigned)i / (unsigned)per : i / per, d = (i - b * per) * V;
-  const Vec<T, V> g = load_vec_nc<T, V>(gate + b * gate_b + d), xv = load_vec_nc<T, V>(x + b * x_b + d);
+  const int64_t row = batch * per <= 0xffffffffll ? (unsigned)i / (unsigned)per : i / per, d = (i - row * per) * V;
+  const Vec<T, V> g = load_vec_nc<T, V>(gate + row * gate_b + d), xv = load_vec_nc<T, V>(x + row * x_b + d);
   bool cut = false;
   if (reset)
-    cut = reset_bytes == 1 ? reinterpret_cast<const uint8_t*>(reset)[b * reset_b] != 0
-                           : reinterpret_cast<const float*>(reset)[b * reset_b] != 0.0f;
-  float* s = state + b * state_b + d;
+    cut = reset_bytes == 1 ? reinterpret_cast<const uint8_t*>(reset)[row * reset_b] != 0
+                           : reinterpret_cast<const float*>(reset)[row * reset_b] != 0.0f;
+  float* s = state + row * state_b + d;
   float h[V];
   if constexpr (V % 4 == 0) {
 #pragma unroll
@@ -401,9 +531,10 @@ __global__ void __launch_bounds__(256)
   Vec<T, V> o;
 #pragma unroll
   for (int k = 0; k < V; k++) {
-    float a, bb, c;
-    coefficients<GATED>(to_f32(g.e[k]), to_f32(xv.e[k]), a, bb, c);
-    h[k] = cut ? bb : fmaf(a, h[k], bb);
+    float a, c;
+    coefficients<GATED>(packed_gate<GATED>(to_f32(g.e[k])), a, c);
+    const float b = GATED ? c * to_f32(xv.e[k]) : to_f32(xv.e[k]);
+    h[k] = cut ? b : fmaf(a, h[k], b);
     o.e[k] = from_f32<T>(h[k]);
   }
   if constexpr (V % 4 == 0) {
@@ -413,7 +544,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int k = 0; k < V; k++) s[k] = h[k];
   }
-  store_vec<T, V>(out + b * out_b + d, o);
+  store_vec<T, V>(out + row * out_b + d, o);
 }
 
 // Warps that keep an SM's loads going; fewer channel groups than this many on every SM and the work is
