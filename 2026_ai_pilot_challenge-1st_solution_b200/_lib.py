@@ -199,7 +199,21 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 def on_device(t):
     """Context in which the tensor's device is the current one (launches go to the current device)."""
-    return _SAME_DEVICE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == t.get_device() else torch.cuda.device(t.device)
+
+
+def raw_stream(t):
+    """stream_of as an integer, without the Python objects on the way (a microsecond of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def checked(t, dtypes, shape, label, like=None):
+    """require_cuda_tensor for the calls whose time is the host's: t has one of ``dtypes``, ``shape`` (None:
+    any) and the device of ``like`` (None: any)."""
+    if (torch.is_tensor(t) and t.dtype in dtypes and (shape is None or t.shape == shape) and t.is_cuda
+            and (like is None or t.get_device() == like.get_device())):
+        return t
+    return require_cuda_tensor(t, dtypes, shape, label, None if like is None else like.device)
 
 
 def require_cuda_tensor(t, dtype, shape, label, device=None):

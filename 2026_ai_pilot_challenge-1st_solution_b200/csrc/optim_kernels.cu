@@ -30,6 +30,7 @@ namespace opt {
 constexpr int THREADS = 256;
 constexpr int QBLOCK = F16_ADAMW_BLOCK;       // values of one scale: a warp's, 8 each
 constexpr int PIECE = THREADS / 32 * QBLOCK;  // values of a block at a time
+constexpr int NORM_PIECE = 4 * PIECE;         // of a block of the norm: eight loads in flight a thread
 static_assert(QBLOCK == 256, "a lane holds two groups of four values of a warp's scale block");
 
 struct Tensor {
@@ -130,50 +131,53 @@ __global__ void __launch_bounds__(THREADS)
   for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
     const int i = tensor_of(tab, piece);
     const T* g = reinterpret_cast<const T*>(tab.t[i].g);
-    const int64_t n = tab.t[i].n, at = (piece - tab.first[i]) * PIECE + threadIdx.x * 4;
+    const int64_t n = tab.t[i].n, at = (piece - tab.first[i]) * NORM_PIECE;
     const bool vec = (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(T) - 1)) == 0;
+    Vec<T, 4> v[8];
+    if (vec && at + NORM_PIECE <= n) {
+#pragma unroll
+      for (int h = 0; h < 8; h++) v[h] = load_vec_nc<T, 4>(g + at + (h * THREADS + threadIdx.x) * 4);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 8; h++) v[h] = load4(g, at + (h * THREADS + threadIdx.x) * 4, n, vec);
+    }
     float q = 0.0f;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const Vec<T, 4> v = load4(g, at + h * (PIECE / 2), n, vec);
+    for (int h = 0; h < 8; h++)
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const float f = to_f32(v.e[k]);
+        const float f = to_f32(v[h].e[k]);
         q = fmaf(f, f, q);
       }
-    }
     sum += (double)q;
   }
   sum = block_sum(sum, s);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
+// x / s rounded towards zero (x >= 0, inv = 1 / s): a Newton step gives the nearest quotient, the sign of its
+// residual says whether that lies above the true one.  What the rounding to a code below looks at are whole
+// units of the quotient's last place, so it decides as the exact quotient would; the nearest one would
+// fall on the wrong side of a code's border once in some 10^6 -- and often where a block's values all
+// shrink alike, which makes the quotients codes again and again.
+__device__ __forceinline__ float quotient_rz(float x, float s, float inv) {
+  const float q0 = x * inv, q = fmaf(fmaf(-q0, s, x), inv, q0);
+  return __int_as_float(__float_as_int(q) - (fmaf(-q, s, x) < 0.0f));
+}
+
 // x >= 0, at most `most`, rounded to `MANT` mantissa bits (subnormals below 2^LOW included): up where
-// the 16 random bits and the part left over carry.  x is fp64, so that the outcome is the one that the
-// moment, its scale and the bits define (a fp32 quotient would fall on the wrong side of a code's
-// border once in some 10^6); what decides lies in the upper word of it.
+// the 16 random bits and the part left over carry.
 template <int MANT, int LOW>
-__device__ __forceinline__ float round_carry(double x, unsigned bits, double most) {
-  constexpr int DROP = 20 - MANT;                 // bits of the upper word's mantissa below a code's
-  const double low = __hiloint2double((1023 + LOW) << 20, 0);
-  x = x > most ? most : x;                        // NaN stays
-  const bool sub = x < low;
-  const int hi = (__double2hiint(sub ? x + low : x) + (int)(bits << (DROP - 16))) & ~((1 << DROP) - 1);
-  const float r = __int_as_float((hi - (896 << 20)) << 3);      // fp64's exponent and mantissa as fp32's
-  return sub ? r - __int_as_float((127 + LOW) << 23) : r;       // in [low, 2 low) a mantissa step is a subnormal one
+__device__ __forceinline__ float round_carry(float x, unsigned bits, float most) {
+  constexpr int DROP = 23 - MANT;
+  const float low = __int_as_float((127 + LOW) << 23);
+  x = fminf(x, most);
+  const bool sub = x < low;                       // in [low, 2 low) a mantissa step is a subnormal one
+  const float y = sub ? __fadd_rz(x, low) : x;
+  const float r = __uint_as_float((__float_as_uint(y) + (bits << (DROP - 16))) & ~((1u << DROP) - 1));
+  return sub ? r - low : r;
 }
 
-// x / s with inv = 1 / s: where the quotient is a fp64 number the product may miss it by its last bit (a
-// block whose values all shrink by the same factor has such quotients, every step), the residual mends it.
-__device__ __forceinline__ double quotient(double x, double s, double inv) {
-  const double q = x * inv;
-  return fma(fma(-q, s, x), inv, q);
-}
-
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a < __int_as_float(0x7f800000) ? a : 0.0f;
-}
 __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
   return v;
@@ -183,6 +187,15 @@ __device__ __forceinline__ float2 unpack8(__nv_fp8x2_storage_t c, __nv_fp8_inter
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(c, kind);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
+
+__device__ __forceinline__ float root_of(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+#define INF __int_as_float(0x7f800000)
+#define NOT_A_NUMBER __int_as_float(0x7fffffff)
 
 template <typename T, int N, int BITS, bool MASTER>
 __global__ void __launch_bounds__(THREADS)
@@ -261,6 +274,7 @@ __global__ void __launch_bounds__(THREADS)
         ms[h][0] = w.x; ms[h][1] = w.y; ms[h][2] = w.z; ms[h][3] = w.w;
       }
     }
+    // past the tensor's end the gradient and the moments are zero, and stay it
     float m_most = 0.0f, v_most = 0.0f;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -278,45 +292,60 @@ __global__ void __launch_bounds__(THREADS)
           now.e[0] = pv[h].e[k];
           w = rounded.r == now.r ? ms[h][k] : w;
         }
-        w = w * hy.decay - rate * m[h][k] / (sqrtf(v[h][k]) * root + hy.eps);
+        // the change is good to some 2^-21 of itself (approximate root and quotient): far below the
+        // parameter's rounding
+        w = fmaf(w, hy.decay, -__fdividef(rate * m[h][k], fmaf(root_of(v[h][k]), root, hy.eps)));
         if (MASTER) ms[h][k] = w;
         pv[h].e[k] = from_f32<T>(w);
-        if (BITS == 8 && e + k < n) {
-          m_most = fmaxf(m_most, finite_abs(m[h][k]));
-          v_most = fmaxf(v_most, finite_abs(v[h][k]));
+        if (BITS == 8) {
+          m_most = fmaxf(m_most, fabsf(m[h][k]));         // a NaN does not count
+          v_most = fmaxf(v_most, v[h][k]);
         }
       }
       store4(p, e, n, vec, pv[h]);
     }
-    double mi = 0.0, vi = 0.0;
+    float mi = 0.0f, vi = 0.0f;
     if (BITS == 8) {
       const float tiny = __int_as_float(1 << 23);       // the smallest normal: its reciprocal is finite
-      m_unit = fmaxf(warp_max(m_most) * (1.0f / 448.0f), tiny);
-      v_unit = fmaxf(warp_max(v_most) * (1.0f / 57344.0f), tiny);
+      m_most = warp_max(m_most);
+      v_most = warp_max(v_most);
+      if (!(m_most < INF) || !(v_most < INF)) {         // an infinity somewhere: the largest finite ones
+        m_most = v_most = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            m_most = fmaxf(m_most, fabsf(m[h][k]) < INF ? fabsf(m[h][k]) : 0.0f);
+            v_most = fmaxf(v_most, v[h][k] < INF ? v[h][k] : 0.0f);
+          }
+        m_most = warp_max(m_most);
+        v_most = warp_max(v_most);
+      }
+      m_unit = fmaxf(m_most * (1.0f / 448.0f), tiny);
+      v_unit = fmaxf(v_most * (1.0f / 57344.0f), tiny);
       if (lane == 0) {
         fl.m_scale[flat / QBLOCK] = m_unit;
         fl.v_scale[flat / QBLOCK] = v_unit;
       }
-      mi = 1.0 / (double)m_unit;
-      vi = 1.0 / (double)v_unit;
+      mi = 1.0f / m_unit;
+      vi = 1.0f / v_unit;
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const int64_t e = at + h * 128 + lane * 4, f = flat + h * 128 + lane * 4;
       if (e >= n) continue;
       if (BITS == 8) {
+        const uint64_t word0 = mix64(key + (uint64_t)(f >> 1)), word1 = mix64(key + (uint64_t)(f >> 1) + 1);
         float mq[4], vq[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const uint64_t word = mix64(key + (uint64_t)((f + k) >> 1));
-          const unsigned bits = (unsigned)(word >> (32 * (k & 1)));
-          const float inf = __int_as_float(0x7f800000), nan = __int_as_float(0x7fffffff);
+          const unsigned bits = (unsigned)((k < 2 ? word0 : word1) >> (32 * (k & 1)));
           const float a = fabsf(m[h][k]), b = v[h][k];
-          const float x = round_carry<3, -6>(quotient(a, m_unit, mi), bits & 0xffff, 448.0);
-          const float y = round_carry<2, -14>(quotient(b, v_unit, vi), bits >> 16, 57344.0);
-          mq[k] = a < inf ? copysignf(x, m[h][k]) : nan;
-          vq[k] = !(b < inf) ? nan : b > 0.0f && y == 0.0f ? 1.52587890625e-05f : y;      // 2^-16, the smallest code
-          if (e + k >= n) mq[k] = vq[k] = 0.0f;
+          const float x = round_carry<3, -6>(quotient_rz(a, m_unit, mi), bits & 0xffff, 448.0f);
+          const float y = round_carry<2, -14>(quotient_rz(b, v_unit, vi), bits >> 16, 57344.0f);
+          mq[k] = a < INF ? copysignf(x, m[h][k]) : NOT_A_NUMBER;
+          // 2^-16, the smallest code, for what is above zero
+          vq[k] = b < INF ? (b > 0.0f ? fmaxf(y, 1.52587890625e-05f) : 0.0f) : NOT_A_NUMBER;
         }
         const uint32_t mc = __nv_cvt_float2_to_fp8x2(make_float2(mq[0], mq[1]), __NV_SATFINITE, __NV_E4M3) |
                             (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(mq[2], mq[3]), __NV_SATFINITE, __NV_E4M3) << 16;
@@ -325,9 +354,6 @@ __global__ void __launch_bounds__(THREADS)
         *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(fl.m) + f) = mc;
         *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(fl.v) + f) = vc;
       } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (e + k >= n) m[h][k] = v[h][k] = 0.0f;
         *reinterpret_cast<float4*>(reinterpret_cast<float*>(fl.m) + f) = make_float4(m[h][0], m[h][1], m[h][2], m[h][3]);
         *reinterpret_cast<float4*>(reinterpret_cast<float*>(fl.v) + f) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
       }
@@ -353,15 +379,18 @@ __global__ void __launch_bounds__(THREADS)
 
 constexpr int BLOCKS_PER_SM = 4;
 
+#undef INF
+#undef NOT_A_NUMBER
+
 template <int N>
-void fill(Table<N>& tab, int count, void* const* p, const void* const* g, const int64_t* n, const int64_t* at,
+void fill(Table<N>& tab, int piece, int count, void* const* p, const void* const* g, const int64_t* n, const int64_t* at,
           const int32_t* index) {
   int64_t pieces = 0;
   for (int i = 0; i < count; i++) {
     tab.t[i] = {p ? p[i] : nullptr, g[i], n[i], at ? at[i] : 0};
     tab.index[i] = index ? index[i] : 0;
     tab.first[i] = pieces;
-    pieces += (n[i] + PIECE - 1) / PIECE;
+    pieces += (n[i] + piece - 1) / piece;
   }
   tab.first[count] = pieces;
   tab.count = count;
@@ -375,7 +404,7 @@ inline unsigned blocks_for(int64_t pieces) {
 template <typename T, int N>
 int squares(int count, const void* const* g, const int64_t* n, double* partial, int room, int* used, cudaStream_t st) {
   Table<N> tab;
-  fill<N>(tab, count, nullptr, g, n, nullptr, nullptr);
+  fill<N>(tab, NORM_PIECE, count, nullptr, g, n, nullptr, nullptr);
   unsigned grid = blocks_for(tab.first[count]);
   if ((int)grid > room) grid = room;
   k_grad_squares<T, N><<<grid, THREADS, 0, st>>>(tab, partial);
@@ -387,7 +416,7 @@ template <typename T, int N>
 int update(int count, void* const* p, const void* const* g, const int64_t* n, const int64_t* at, const int32_t* index,
            const Hyper& hy, const Flat& fl, int bits, cudaStream_t st) {
   Table<N> tab;
-  fill<N>(tab, count, p, g, n, at, index);
+  fill<N>(tab, PIECE, count, p, g, n, at, index);
   const unsigned grid = blocks_for(tab.first[count]);
   const auto go = [&](auto k) { k<<<grid, THREADS, 0, st>>>(tab, hy, fl); };
   if constexpr (sizeof(T) == 4) {

@@ -15,6 +15,9 @@ import torch
 from . import _lib
 
 
+_FLOATS = tuple(_lib.DTYPES)
+
+
 def _rows(x):
     """x as (rows, dim) with unit column stride (a view where its layout allows)."""
     x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
@@ -25,30 +28,29 @@ def _row_stride(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+def _forward(x, rows, weight, bias, eps, stats):
+    n, dim = rows.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if n:
+        wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+        at = stats.data_ptr() if stats is not None else None
+        with _lib.on_device(x):
+            _lib.check(_lib.load().f16_layer_norm_fwd(
+                rows.data_ptr(), n, dim, _row_stride(rows), _lib.DTYPES[x.dtype],
+                weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None,
+                _lib.DTYPES[wdtype], eps, y.data_ptr(), dim, at, at + 4 * n if at is not None else None,
+                _lib.raw_stream(x)), "f16_layer_norm_fwd")
+    return y
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows = _rows(x)
-        n, dim = rows.shape
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = None
-        if any(ctx.needs_input_grad):
-            stats = torch.empty(2, n, dtype=torch.float32, device=x.device)
-        wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-        if weight is not None:
-            weight = weight.contiguous()
-        if bias is not None:
-            bias = bias.contiguous()
-        if n:
-            with _lib.on_device(x):
-                _lib.check(_lib.load().f16_layer_norm_fwd(
-                    rows.data_ptr(), n, dim, _row_stride(rows), _lib.DTYPES[x.dtype], _lib.ptr(weight),
-                    _lib.ptr(bias), _lib.DTYPES[wdtype], eps, y.data_ptr(), dim,
-                    stats.data_ptr() if stats is not None else None,
-                    stats.data_ptr() + 4 * n if stats is not None else None, _lib.stream_of(x)), "f16_layer_norm_fwd")
-        ctx.wdtype = wdtype
+        stats = torch.empty(2, rows.shape[0], dtype=torch.float32, device=x.device)
+        ctx.wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
         ctx.save_for_backward(rows, weight, stats)
-        return y
+        return _forward(x, rows, weight, bias, eps, stats)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -66,29 +68,36 @@ class _LayerNorm(torch.autograd.Function):
         db = torch.empty(dim, dtype=ctx.wdtype, device=x.device) if need_b else None
         lib = _lib.load()
         with _lib.on_device(x):
-            room = int(lib.f16_layer_norm_scratch_floats(n, dim)) if need_w or need_b else 0
+            room = lib.f16_layer_norm_scratch_floats(n, dim) if need_w or need_b else 0
             scratch = torch.empty(room, dtype=torch.float32, device=x.device) if room else None
+            at = stats.data_ptr()
             _lib.check(lib.f16_layer_norm_bwd(
                 dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), n, dim, _lib.DTYPES[x.dtype],
-                _lib.ptr(weight), _lib.DTYPES[ctx.wdtype], stats.data_ptr(), stats.data_ptr() + 4 * n, _lib.ptr(dx), dim,
-                _lib.ptr(dw), _lib.ptr(db), _lib.ptr(scratch), room, _lib.stream_of(x)), "f16_layer_norm_bwd")
+                weight.data_ptr() if weight is not None else None, _lib.DTYPES[ctx.wdtype], at, at + 4 * n,
+                dx.data_ptr() if need_x else None, dim, dw.data_ptr() if need_w else None,
+                db.data_ptr() if need_b else None, scratch.data_ptr() if room else None, room,
+                _lib.raw_stream(x)), "f16_layer_norm_bwd")
         return dx, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (module docstring)."""
-    _lib.require_cuda_tensor(x, tuple(_lib.DTYPES), None, "layer_norm input")
+    _lib.checked(x, _FLOATS, None, "layer_norm input")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("layer_norm needs a last axis of at least one value")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    dim = x.shape[-1]
-    for t, name in ((weight, "layer_norm weight"), (bias, "layer_norm bias")):
-        if t is not None:
-            _lib.require_cuda_tensor(t, (torch.float32, x.dtype), (dim,), name, x.device)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError("layer_norm weight and bias must have the same dtype")
-    return _LayerNorm.apply(x, weight, bias, float(eps))
+    shape = x.shape[-1:]
+    if weight is not None:
+        weight = _lib.checked(weight, (torch.float32, x.dtype), shape, "layer_norm weight", x).contiguous()
+    if bias is not None:
+        bias = _lib.checked(bias, (torch.float32, x.dtype), shape, "layer_norm bias", x).contiguous()
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError("layer_norm weight and bias must have the same dtype")
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                    or bias is not None and bias.requires_grad):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _forward(x, _rows(x), weight, bias, float(eps), None)
 
 
 class LayerNorm(torch.nn.LayerNorm):

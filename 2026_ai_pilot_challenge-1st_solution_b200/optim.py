@@ -20,6 +20,7 @@ Moments, masters and step counts of a group's tensors of one type lie in flat bu
 (``state_buffers``); ``state[p]`` holds the tensors' views of them.
 """
 import ctypes as C
+import operator
 
 import torch
 
@@ -27,6 +28,11 @@ from . import _lib
 
 BLOCK = 256                     # F16_ADAMW_BLOCK: values that share a scale
 LAUNCH_TENSORS, LAUNCH_PARTIALS = 720, 592      # tensors of one launch, and the partial sums it may write
+
+
+_grad, _layout, _dtype = (operator.attrgetter(name) for name in ("grad", "layout", "dtype"))
+_numel, _device, _contiguous, _address = (torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous,
+                                          torch.Tensor.data_ptr)
 
 
 class _Bucket:
@@ -53,6 +59,7 @@ class _Bucket:
             self.buffers["master"] = zeros(total, torch.float32)
         self.buffers["step"] = zeros(len(params), torch.int64)
         self.ticket = zeros(1, torch.int32)
+        self.prepare(bits)
 
     def views(self, i):
         """The state of tensor i: views of the flat buffers."""
@@ -67,40 +74,49 @@ class _Bucket:
                 out[name] = flat[first:first + n].view(self.params[i].shape)
         return out
 
-    def arguments(self, bits):
-        """(AdamwArgs with the table of the tensors that have a gradient, what it points to), or None."""
-        live = [i for i, p in enumerate(self.params) if p.grad is not None and p.numel()]
-        if not live:
-            return None
-        n = len(live)
-        params, grads, keep = [], [], []
-        for i in live:
-            p, g = self.params[i], self.params[i].grad
-            if g.is_sparse:
-                raise RuntimeError("AdamW does not take sparse gradients")
-            if p.dtype != self.dtype or p.device != self.device or not p.is_contiguous():
-                raise RuntimeError("a parameter's type, device or layout changed after the optimiser was made")
-            if g.dtype != self.dtype or g.device != self.device:
-                raise TypeError(f"a gradient must be {self.dtype} on {self.device} as its parameter is")
-            if not g.is_contiguous():
-                g = g.contiguous()
-            keep.append(g)
-            params.append(p.data_ptr())
-            grads.append(g.data_ptr())
-        a = _lib.AdamwArgs()
-        arrays = ((C.c_void_p * n)(*params), (C.c_void_p * n)(*grads),
-                  (C.c_int64 * n)(*[self.params[i].numel() for i in live]),
-                  (C.c_int64 * n)(*[self.firsts[i] for i in live]), (C.c_int32 * n)(*live))
-        a.count, a.dtype, a.state_bits = n, _lib.DTYPES[self.dtype], bits
-        a.params_host, a.grads_host, a.numel_host, a.first_host, a.index_host = (C.addressof(x) for x in arrays)
+    def prepare(self, bits):
+        """What every step's call has alike: the table of all tensors, and the flat buffers' addresses."""
+        self.numels = [p.numel() for p in self.params]
+        n = len(self.params)
+        self.tables = ((C.c_void_p * n)(), (C.c_void_p * n)(), (C.c_int64 * n)(), (C.c_int64 * n)(), (C.c_int32 * n)())
         b = self.buffers
-        a.exp_avg, a.exp_avg_sq = b["exp_avg"].data_ptr(), b["exp_avg_sq"].data_ptr()
-        if bits == 8:
-            a.exp_avg_scale, a.exp_avg_sq_scale = b["exp_avg_scale"].data_ptr(), b["exp_avg_sq_scale"].data_ptr()
-        if "master" in b:
-            a.master = b["master"].data_ptr()
-        a.steps, a.ticket = b["step"].data_ptr(), self.ticket.data_ptr()
-        return a, (arrays, keep, [self.params[i] for i in live])
+        at = lambda name: b[name].data_ptr() if name in b else None
+        self.args = _lib.AdamwArgs(0, _lib.DTYPES[self.dtype], bits, *(C.addressof(t) for t in self.tables), 0, 0, 0, 0, 0,
+                                   0, at("exp_avg"), at("exp_avg_sq"), at("exp_avg_scale"), at("exp_avg_sq_scale"),
+                                   at("master"), at("step"), self.ticket.data_ptr())
+        self.tabled = None          # the tensors that the last three tables hold
+
+    def arguments(self):
+        """(AdamwArgs whose tables hold the tensors with a gradient, these tensors, what has to stay alive until
+        the launch), or None."""
+        # maps over method descriptors: a step over hundreds of small tensors is bound by this loop
+        params, numels, grads = self.params, self.numels, list(map(_grad, self.params))
+        live = range(len(params))
+        if type(None) in set(map(type, grads)) or 0 in numels:
+            live = [i for i, g in enumerate(grads) if g is not None and numels[i]]
+            if not live:
+                return None
+            params, grads, numels = [params[i] for i in live], [grads[i] for i in live], [numels[i] for i in live]
+        both = params + grads
+        if set(map(_layout, grads)) != {torch.strided}:
+            raise RuntimeError("AdamW does not take sparse gradients")
+        if (list(map(_numel, both)) != numels + numels or set(map(_dtype, both)) != {self.dtype}
+                or set(map(_device, both)) != {self.device.index} or not all(map(_contiguous, params))):
+            raise RuntimeError("a parameter's or a gradient's size, type, device or layout is not what it was when the "
+                               "optimiser was made")
+        if not all(map(_contiguous, grads)):
+            grads = [g.detach().contiguous() for g in grads]
+        n = len(live)
+        t = self.tables
+        t[0][:n] = list(map(_address, params))
+        t[1][:n] = list(map(_address, grads))
+        if live != self.tabled:
+            t[2][:n] = numels
+            t[3][:n] = [self.firsts[i] for i in live]
+            t[4][:n] = live
+            self.tabled = live
+        self.args.count = n
+        return self.args, params, grads
 
 
 class AdamW(torch.optim.Optimizer):
@@ -160,6 +176,9 @@ class AdamW(torch.optim.Optimizer):
             for i, p in enumerate(b.params):
                 self.state[p] = b.views(i)
 
+    def __getstate__(self):
+        raise TypeError("AdamW is not copied or pickled; make a new one and load_state_dict into it")
+
     def state_buffers(self):
         """The flat buffers behind the state, one dict for each group and parameter type: "exp_avg",
         "exp_avg_sq" (with "_scale" each for 8-bit states), "master" where there are masters, "step".
@@ -187,7 +206,6 @@ class AdamW(torch.optim.Optimizer):
             for n, t in self.state[p].items():
                 t.zero_() if new is None else t.copy_(new[n])
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One step over every parameter with a gradient; returns the closure's loss, if any."""
         loss = None
@@ -198,32 +216,30 @@ class AdamW(torch.optim.Optimizer):
         for group, buckets in zip(self.param_groups, self._buckets):
             self._check_numbers(group)
             for b in buckets:
-                made = b.arguments(self.state_bits)
+                made = b.arguments()
                 if made is not None:
                     calls.append((group, b, *made))
         if not calls:
             return loss
         lib = _lib.load()
-        device = calls[0][1].buffers["step"]
+        device = calls[0][1].ticket
         with _lib.on_device(device):
-            stream = _lib.stream_of(device)
-            partial, used = None, 0
+            stream = _lib.raw_stream(device)
+            partial, norm, used = None, None, 0
             if self.max_grad_norm is not None:
-                room = sum(-(-a.count // LAUNCH_TENSORS) for _, _, a, _ in calls) * LAUNCH_PARTIALS
-                partial = torch.empty(room, dtype=torch.float64, device=device.device)
+                room = sum([-(-a.count // LAUNCH_TENSORS) for _, _, a, _, _ in calls]) * LAUNCH_PARTIALS
+                sums = torch.empty(room, dtype=torch.float64, device=device.device)
+                partial = sums.data_ptr()
                 self.grad_norm = torch.empty((), dtype=torch.float32, device=device.device)
-                for _, _, a, _ in calls:
-                    n = C.c_int(0)
-                    _lib.check(lib.f16_grad_squares(a.count, a.grads_host, a.numel_host, a.dtype,
-                                                    partial.data_ptr() + 8 * used, room - used, C.byref(n), stream),
-                               "f16_grad_squares")
+                norm, n = self.grad_norm.data_ptr(), C.c_int(0)
+                for _, _, a, _, _ in calls:
+                    _lib.check(lib.f16_grad_squares(a.count, a.grads_host, a.numel_host, a.dtype, partial + 8 * used,
+                                                    room - used, C.byref(n), stream), "f16_grad_squares")
                     used += n.value
-            for group, _, a, (_, _, params) in calls:
-                a.lr, a.eps, a.weight_decay = float(group["lr"]), float(group["eps"]), float(group["weight_decay"])
+            for group, _, a, params, _ in calls:
+                a.lr, a.eps, a.weight_decay = group["lr"], group["eps"], group["weight_decay"]
                 a.beta1, a.beta2 = group["betas"]
-                if partial is not None:
-                    a.max_norm, a.partial, a.partials = float(self.max_grad_norm), partial.data_ptr(), used
-                    a.norm = self.grad_norm.data_ptr()
+                a.max_norm, a.partial, a.partials, a.norm = self.max_grad_norm or 0.0, partial, used, norm
                 a.seed = self.seed
                 _lib.check(lib.f16_adamw_step(C.byref(a), stream), "f16_adamw_step")
                 torch.autograd.graph.increment_version(params)      # written behind autograd's back

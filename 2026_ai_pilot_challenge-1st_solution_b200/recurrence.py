@@ -34,51 +34,49 @@ def _like(x):
     return out if out.stride(2) == 1 or x.shape[2] == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def _fill(args, name, t):
-    setattr(args, name, t.data_ptr())
-    setattr(args, name + "_t", t.stride(0))
-    setattr(args, name + "_b", t.stride(1))
+_FLOATS, _FLAGS, _F32, _I64 = tuple(_lib.DTYPES), (torch.bool, torch.uint8, torch.float32), (torch.float32,), (torch.int64,)
 
 
-def _args(gate, x, h0, reset, lengths, gated):
-    a = _lib.ScanArgs()
-    a.dtype, a.gated = _lib.DTYPES[x.dtype], int(gated)
-    a.steps, a.batch, a.dim = x.shape
-    _fill(a, "gate", gate)
-    _fill(a, "x", x)
-    if h0 is not None:
-        a.h0 = h0.data_ptr()
-    if reset is not None:
-        a.reset, a.reset_bytes = reset.data_ptr(), reset.element_size()
-        a.reset_t, a.reset_b = reset.stride(0), reset.stride(1)
-    if lengths is not None:
-        a.lengths = lengths.data_ptr()
-    return a
+def _place(t):
+    """(address, time stride, batch stride) of a sequence tensor or None."""
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _args(gate, x, h0, reset, lengths, gated, h, hn, saved, dh=None, dhn=None, dgate=None, dx=None, dh0=None):
+    return _lib.ScanArgs(_lib.DTYPES[x.dtype], gated, *x.shape, *_place(gate), *_place(x), _at(h0), _at(reset),
+                         reset.element_size() if reset is not None else 0,
+                         *(reset.stride() if reset is not None else (0, 0)), _at(lengths), *_place(h), _at(hn), _at(saved),
+                         *_place(dh), _at(dhn), *_place(dgate), *_place(dx), _at(dh0))
+
+
+def _forward(gate, x, h0, reset, lengths, gated, keep):
+    """(h, hn, the states that the backward pass needs if ``keep``); gate and x with unit stride along dim."""
+    steps, batch, dim = x.shape
+    h = _like(x)
+    hn = torch.empty(batch, dim, dtype=torch.float32, device=x.device)
+    saved = None
+    if not x.numel():
+        hn.zero_() if h0 is None else hn.copy_(h0)
+    else:
+        lib = _lib.load()
+        if keep:
+            saved = torch.empty(lib.f16_scan_saved_floats(steps, batch, dim), dtype=torch.float32, device=x.device)
+        a = _args(gate, x, h0, reset, lengths, gated, h, hn, saved)
+        with _lib.on_device(x):
+            _lib.check(lib.f16_scan_fwd(C.byref(a), _lib.raw_stream(x)), "f16_scan_fwd")
+    return h, hn, saved
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, reset, lengths, gated):
         ctx.set_materialize_grads(False)
-        steps, batch, dim = x.shape
         gate, x = _strided(gate), _strided(x)
-        h = _like(x)
-        hn = torch.empty(batch, dim, dtype=torch.float32, device=x.device)
-        if h0 is not None:
-            h0 = h0.contiguous()
-        saved = None
-        if x.numel() == 0:
-            hn.zero_() if h0 is None else hn.copy_(h0)
-        else:
-            lib = _lib.load()
-            a = _args(gate, x, h0, reset, lengths, gated)
-            _fill(a, "h", h)
-            a.hn = hn.data_ptr()
-            if any(ctx.needs_input_grad[:3]):
-                saved = torch.empty(lib.f16_scan_saved_floats(steps, batch, dim), dtype=torch.float32, device=x.device)
-                a.saved = saved.data_ptr()
-            with _lib.on_device(x):
-                _lib.check(lib.f16_scan_fwd(C.byref(a), _lib.stream_of(x)), "f16_scan_fwd")
+        h, hn, saved = _forward(gate, x, h0, reset, lengths, gated, True)
         ctx.gated = gated
         ctx.save_for_backward(gate, x, h0, reset, lengths, saved)
         return h, hn
@@ -86,56 +84,39 @@ class _Scan(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dhn):
-        gate, x, h0, reset, lengths, saved = ctx.saved_tensors
         if dh is None and dhn is None:
             return None, None, None, None, None, None
+        gate, x, h0, reset, lengths, saved = ctx.saved_tensors
         need_gate, need_x, need_h0 = ctx.needs_input_grad[:3]
-        batch, dim = x.shape[1:]
         dgate = _like(gate) if need_gate else None
         dx = _like(x) if need_x else None
-        dh0 = torch.empty(batch, dim, dtype=torch.float32, device=x.device) if need_h0 else None
-        if x.numel() == 0:
+        dh0 = torch.empty(x.shape[1:], dtype=torch.float32, device=x.device) if need_h0 else None
+        if not x.numel():
             if dh0 is not None:
                 dh0.zero_() if dhn is None else dh0.copy_(dhn)
             return dgate, dx, dh0, None, None, None
-        a = _args(gate, x, h0, reset, lengths, ctx.gated)
-        a.saved = saved.data_ptr()
-        if dh is not None:
-            dh = _strided(dh)
-            _fill(a, "dh", dh)
-        if dhn is not None:
-            dhn = dhn.contiguous()
-            a.dhn = dhn.data_ptr()
-        if dgate is not None:
-            _fill(a, "dgate", dgate)
-        if dx is not None:
-            _fill(a, "dx", dx)
-        if dh0 is not None:
-            a.dh0 = dh0.data_ptr()
+        dh = _strided(dh) if dh is not None else None
+        dhn = dhn.contiguous() if dhn is not None else None
+        a = _args(gate, x, h0, reset, lengths, ctx.gated, None, None, saved, dh, dhn, dgate, dx, dh0)
         with _lib.on_device(x):
-            _lib.check(_lib.load().f16_scan_bwd(C.byref(a), _lib.stream_of(x)), "f16_scan_bwd")
+            _lib.check(_lib.load().f16_scan_bwd(C.byref(a), _lib.raw_stream(x)), "f16_scan_bwd")
         return dgate, dx, dh0, None, None, None
 
 
-def _flags(reset, shape, device):
-    _lib.require_cuda_tensor(reset, (torch.bool, torch.uint8, torch.float32), shape, "reset flags", device)
-    return reset
-
-
 def _scan(gate, x, h0, reset, lengths, gated, name):
-    _lib.require_cuda_tensor(x, tuple(_lib.DTYPES), None, f"{name} input")
+    _lib.checked(x, _FLOATS, None, f"{name} input")
     if x.dim() != 3:
         raise ValueError(f"{name} takes (steps, batch, dim) tensors")
-    _lib.require_cuda_tensor(gate, x.dtype, x.shape, "gate" if gated else "coefficients", x.device)
-    steps, batch, dim = x.shape
+    _lib.checked(gate, (x.dtype,), x.shape, "gate" if gated else "coefficients", x)
     if h0 is not None:
-        _lib.require_cuda_tensor(h0, torch.float32, (batch, dim), "initial state", x.device)
+        h0 = _lib.checked(h0, _F32, x.shape[1:], "initial state", x).contiguous()
     if reset is not None:
-        _flags(reset, (steps, batch), x.device)
+        _lib.checked(reset, _FLAGS, x.shape[:2], "reset flags", x)
     if lengths is not None:
-        _lib.require_cuda_tensor(lengths, torch.int64, (batch,), "lengths", x.device)
-        lengths = lengths.contiguous()
-    return _Scan.apply(gate, x, h0, reset, lengths, gated)
+        lengths = _lib.checked(lengths, _I64, x.shape[1:2], "lengths", x).contiguous()
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or h0 is not None and h0.requires_grad):
+        return _Scan.apply(gate, x, h0, reset, lengths, int(gated))
+    return _forward(_strided(gate), _strided(x), h0, reset, lengths, int(gated), False)[:2]
 
 
 def gated_scan(gate, x, h0=None, reset=None, lengths=None):
@@ -156,36 +137,35 @@ def linear_scan(a, x, h0=None, reset=None, lengths=None):
     return _scan(a, x, h0, reset, lengths, False, "linear_scan")
 
 
-@torch.no_grad()
 def _step(gate, x, state, reset, out, gated, name):
-    _lib.require_cuda_tensor(x, tuple(_lib.DTYPES), None, f"{name} input")
+    _lib.checked(x, _FLOATS, None, f"{name} input")
     if x.dim() != 2:
         raise ValueError(f"{name} takes (batch, dim) tensors")
-    _lib.require_cuda_tensor(gate, x.dtype, x.shape, "gate" if gated else "coefficients", x.device)
-    _lib.require_cuda_tensor(state, torch.float32, x.shape, "state", x.device)
-    batch, dim = x.shape
+    shape = x.shape
+    _lib.checked(gate, (x.dtype,), shape, "gate" if gated else "coefficients", x)
+    _lib.checked(state, _F32, shape, "state", x)
     if out is None:
-        out = torch.empty(batch, dim, dtype=x.dtype, device=x.device)
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
     else:
-        _lib.require_cuda_tensor(out, x.dtype, x.shape, "output", x.device)
-    for t, label in ((state, "state"), (out, "output")):
-        if batch and dim and (dim > 1 and t.stride(1) != 1 or batch > 1 and t.stride(0) < dim):
-            raise ValueError(f"{label} rows must be contiguous and apart")
+        _lib.checked(out, (x.dtype,), shape, "output", x)
     if reset is not None:
-        _flags(reset, (batch,), x.device)
-    if x.numel() == 0:
+        _lib.checked(reset, _FLAGS, shape[:1], "reset flags", x)
+    batch, dim = shape
+    if not batch or not dim:
         return out
+    for t, label in ((state, "state"), (out, "output")):
+        if not t.is_contiguous() and (dim > 1 and t.stride(1) != 1 or batch > 1 and t.stride(0) < dim):
+            raise ValueError(f"{label} rows must be contiguous and apart")
     if dim > 1:
         gate = gate if gate.stride(1) == 1 else gate.contiguous()
         x = x if x.stride(1) == 1 else x.contiguous()
-    rows = lambda t: t.stride(0) if batch > 1 else dim
+    rows = [t.stride(0) if batch > 1 else dim for t in (gate, x, state, out)]
     with _lib.on_device(x):
         _lib.check(_lib.load().f16_scan_step(
-            gate.data_ptr(), rows(gate), x.data_ptr(), rows(x), batch, dim, _lib.DTYPES[x.dtype], int(gated),
-            _lib.ptr(reset), reset.element_size() if reset is not None else 0,
-            reset.stride(0) if reset is not None else 0, state.data_ptr(), rows(state), out.data_ptr(), rows(out),
-            _lib.stream_of(x)), "f16_scan_step")
-    torch.autograd.graph.increment_version((state, out))
+            gate.data_ptr(), rows[0], x.data_ptr(), rows[1], batch, dim, _lib.DTYPES[x.dtype], gated, _at(reset),
+            reset.element_size() if reset is not None else 0, reset.stride(0) if reset is not None else 0,
+            state.data_ptr(), rows[2], out.data_ptr(), rows[3], _lib.raw_stream(x)), "f16_scan_step")
+    torch.autograd.graph.increment_version((state, out))      # written behind autograd's back
     return out
 
 
@@ -193,9 +173,9 @@ def gated_step(gate, x, state, reset=None, out=None):
     """One step of ``gated_scan`` for a decision: gate, x (batch, dim), state (batch, dim) fp32 updated in
     place, reset (batch,) flags or None.  Returns the new state in the inputs' type (``out``); no
     gradient is recorded."""
-    return _step(gate, x, state, reset, out, True, "gated_step")
+    return _step(gate, x, state, reset, out, 1, "gated_step")
 
 
 def linear_step(a, x, state, reset=None, out=None):
     """One step of ``linear_scan``; arguments as in ``gated_step``."""
-    return _step(a, x, state, reset, out, False, "linear_step")
+    return _step(a, x, state, reset, out, 0, "linear_step")

@@ -359,6 +359,8 @@ def test_state_dict_round_trip(cuda, bits):
         wrong.load_state_dict(opt.state_dict())
     with pytest.raises(ValueError):
         opt_mod.AdamW(b[:2]).load_state_dict(opt.state_dict())
+    with pytest.raises(TypeError):
+        copy.deepcopy(opt)
 
 
 @pytest.mark.parametrize("bits", [32, 8])
@@ -410,6 +412,25 @@ def test_odd_gradients(cuda):
     opt_mod.AdamW([p, e]).step()
     opt_mod.AdamW([q]).step()
     assert torch.equal(p, q)
+
+
+def test_changed_parameters_are_refused(cuda):
+    """Storage swapped for one of another size, type or layout is not written over; of the same form it is
+    followed."""
+    opt_mod = pkg_module("optim")
+    for new in (torch.ones(9, 4, device=cuda), torch.ones(6, 4, device=cuda).half(), torch.ones(4, 6, device=cuda).t()):
+        p = torch.ones(6, 4, device=cuda, requires_grad=True)
+        p.grad = torch.ones_like(p)
+        opt = opt_mod.AdamW([p])
+        p.data = new
+        with pytest.raises((RuntimeError, TypeError)):
+            opt.step()
+    p = torch.ones(6, 4, device=cuda, requires_grad=True)
+    p.grad = torch.ones_like(p)
+    opt = opt_mod.AdamW([p], lr=0.5, weight_decay=0.0)
+    p.data = torch.full((6, 4), 3.0, device=cuda)
+    opt.step()
+    assert bool((p - 2.5).abs().max() < 1e-5)
 
 
 def test_refusals(cuda):
