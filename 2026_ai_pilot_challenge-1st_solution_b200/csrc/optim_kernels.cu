@@ -28,6 +28,9 @@ namespace f16 {
 namespace opt {
 
 constexpr int THREADS = 256;
+// Resident update blocks, each walking over its share: 64 registers a thread, 80 for 8-bit moments.
+__host__ __device__ constexpr int blocks_per_sm(int bits) { return bits == 8 ? 3 : 4; }
+constexpr int NORM_BLOCKS_PER_SM = 4;
 constexpr int QBLOCK = F16_ADAMW_BLOCK;       // values of one scale: a warp's, 8 each
 constexpr int PIECE = THREADS / 32 * QBLOCK;  // values of a block at a time
 constexpr int NORM_PIECE = 4 * PIECE;         // of a block of the norm: eight loads in flight a thread
@@ -53,7 +56,7 @@ static_assert(sizeof(Table<LARGE>) + 256 <= 32764, "kernel parameters");
 
 struct Hyper {
   double lr, b1, b2;
-  float eps, decay;                 // decay: 1 - lr wd
+  float eps, decay, minus_zero;     // decay: 1 - lr wd
   float keep1, new1, keep2, new2;   // b1, 1 - b1, b2, 1 - b2, each rounded from fp64
   double max_norm;
 };
@@ -160,27 +163,51 @@ __global__ void __launch_bounds__(THREADS)
 // units of the quotient's last place, so it decides as the exact quotient would; the nearest one would
 // fall on the wrong side of a code's border once in some 10^6 -- and often where a block's values all
 // shrink alike, which makes the quotients codes again and again.
-__device__ __forceinline__ float quotient_rz(float x, float s, float inv) {
-  const float q0 = x * inv, q = fmaf(fmaf(-q0, s, x), inv, q0);
-  return __int_as_float(__float_as_int(q) - (fmaf(-q, s, x) < 0.0f));
+__device__ __forceinline__ Two quotient_rz(Two x, Two minus_s, Two inv) {
+  const Two q0 = x * inv, q = fma2(fma2(q0, minus_s, x), inv, q0);
+  const float2 f = split(q), res = split(fma2(q, minus_s, x));
+  return two(__int_as_float(__float_as_int(f.x) + (__float_as_int(res.x) >> 31)),
+             __int_as_float(__float_as_int(f.y) + (__float_as_int(res.y) >> 31)));
 }
 
-// x >= 0, at most `most`, rounded to `MANT` mantissa bits (subnormals below 2^LOW included): up where
-// the 16 random bits and the part left over carry.
+// x >= 0 rounded to `MANT` mantissa bits (subnormals below 2^LOW included): up where the 16 random bits
+// and the part left over carry.  A carry above the type's largest is taken back by the conversion to it,
+// which saturates.
 template <int MANT, int LOW>
-__device__ __forceinline__ float round_carry(float x, unsigned bits, float most) {
+__device__ __forceinline__ float round_carry(float x, unsigned bits) {
   constexpr int DROP = 23 - MANT;
   const float low = __int_as_float((127 + LOW) << 23);
-  x = fminf(x, most);
-  const bool sub = x < low;                       // in [low, 2 low) a mantissa step is a subnormal one
-  const float y = sub ? __fadd_rz(x, low) : x;
-  const float r = __uint_as_float((__float_as_uint(y) + (bits << (DROP - 16))) & ~((1u << DROP) - 1));
-  return sub ? r - low : r;
+  const bool sub = x < low;
+  if (sub) x = __fadd_rz(x, low);                 // in [low, 2 low) a mantissa step is a subnormal one
+  float r = __uint_as_float((__float_as_uint(x) + (bits << (DROP - 16))) & ~((1u << DROP) - 1));
+  if (sub) r -= low;
+  return r;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  return v;
+constexpr unsigned INF_BITS = 0x7f800000u;        // of sizes as integers: finite < infinite < NaN
+
+// The moments' sizes that make their block's scales: the largest finite ones, as integers.
+__device__ __forceinline__ void block_sizes(const Two (&m)[2][2], const Two (&v)[2][2], unsigned& m_most,
+                                            unsigned& v_most, bool& finite) {
+  const auto most = [](const Two (&t)[2][2], unsigned below) {
+    unsigned a = 0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const float2 f = split(t[h][k]);
+        const unsigned x = __float_as_uint(f.x) & 0x7fffffffu, y = __float_as_uint(f.y) & 0x7fffffffu;
+        a = max(a, max(x < below ? x : 0u, y < below ? y : 0u));
+      }
+    return __reduce_max_sync(~0u, a);
+  };
+  m_most = most(m, 0xffffffffu);
+  v_most = most(v, 0xffffffffu);
+  finite = m_most < INF_BITS && v_most < INF_BITS;
+  if (!finite) {
+    m_most = most(m, INF_BITS);
+    v_most = most(v, INF_BITS);
+  }
 }
 
 __device__ __forceinline__ float2 unpack8(__nv_fp8x2_storage_t c, __nv_fp8_interpretation_t kind) {
@@ -194,30 +221,180 @@ __device__ __forceinline__ float root_of(float v) {
   return r;
 }
 
-#define INF __int_as_float(0x7f800000)
-#define NOT_A_NUMBER __int_as_float(0x7fffffff)
+// What a step's update of one tensor needs beside its values.
+struct Numbers {
+  float clip, rate, root;       // of the gradient; lr / (1 - b1^t); 1 / sqrt(1 - b2^t)
+  uint64_t key;
+};
+
+// The parameter after the step.  The change is good to some 2^-21 of itself (approximate root and
+// reciprocal): far below the parameter's rounding.
+__device__ __forceinline__ float changed(float w, float m, float v, const Hyper& hy, const Numbers& nu) {
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root_of(v), nu.root, hy.eps)));
+  return fmaf(-(nu.rate * m), inv, w * hy.decay);
+}
+
+template <typename T>
+__device__ __forceinline__ bool same(T a, T b) {
+  Vec<T, 1> x, y;
+  x.e[0] = a;
+  y.e[0] = b;
+  return x.r == y.r;
+}
+
+// A warp's QBLOCK values from element `at` of a tensor on.  FULL: all of them exist, aligned for loads of
+// four.  Else the gradient, the moments and the master are zero past the tensor's end, and stay it.
+template <typename T, int BITS, bool MASTER, bool FULL>
+__device__ __forceinline__ void update_block(T* p, const T* g, int64_t n, int64_t at, int64_t flat, bool vec,
+                                             const Hyper& hy, const Flat& fl, const Numbers& nu) {
+  const int lane4 = (threadIdx.x & 31) * 4;
+  Vec<T, 4> pv[2], gv[2];
+  Two m[2][2], v[2][2];
+  float ms[2][4];
+  float m_unit = 0.0f, v_unit = 0.0f;
+  if (FULL) {
+    p += at + lane4;
+    g += at + lane4;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    gv[h] = FULL ? load_vec_nc<T, 4>(g + h * 128) : load4(g, at + h * 128 + lane4, n, vec);
+    pv[h] = FULL ? load_vec<T, 4>(p + h * 128) : load4<T>(p, at + h * 128 + lane4, n, vec);
+  }
+  if (BITS == 8) {
+    const uint32_t* mp = reinterpret_cast<const uint32_t*>(reinterpret_cast<uint8_t*>(fl.m) + flat + lane4);
+    const uint32_t* vp = reinterpret_cast<const uint32_t*>(reinterpret_cast<uint8_t*>(fl.v) + flat + lane4);
+    const uint32_t mc[2] = {mp[0], mp[32]}, vc[2] = {vp[0], vp[32]};
+    m_unit = fl.m_scale[flat / QBLOCK];
+    v_unit = fl.v_scale[flat / QBLOCK];
+    const Two mu = two(m_unit), vu = two(v_unit);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const float2 a = unpack8(mc[h] >> (16 * k) & 0xffff, __NV_E4M3), b = unpack8(vc[h] >> (16 * k) & 0xffff, __NV_E5M2);
+        m[h][k] = two(a.x, a.y) * mu;
+        v[h][k] = two(b.x, b.y) * vu;
+      }
+  } else {
+    const float4* mp = reinterpret_cast<const float4*>(reinterpret_cast<float*>(fl.m) + flat + lane4);
+    const float4* vp = reinterpret_cast<const float4*>(reinterpret_cast<float*>(fl.v) + flat + lane4);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const float4 a = mp[32 * h], b = vp[32 * h];
+      m[h][0] = two(a.x, a.y);
+      m[h][1] = two(a.z, a.w);
+      v[h][0] = two(b.x, b.y);
+      v[h][1] = two(b.z, b.w);
+    }
+  }
+  float4* wp = reinterpret_cast<float4*>(fl.master + flat + lane4);
+  if (MASTER) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) *reinterpret_cast<float4*>(ms[h]) = wp[32 * h];
+  }
+  const Two zero = two(hy.minus_zero), clip = two(nu.clip), keep1 = two(hy.keep1), new1 = two(hy.new1), keep2 = two(hy.keep2), new2 = two(hy.new2);
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const Two gr = pair_of<T, 4>(gv[h], k) * clip;
+      // each product rounded by itself, as torch's expressions do (a product and a sum of pairs are made one
+      // fused operation by the assembler; with a zero added that it does not know the product stays)
+      m[h][k] = fma2(keep1, m[h][k], zero) + fma2(new1, gr, zero);
+      v[h][k] = fma2(keep2, v[h][k], zero) + fma2(new2, fma2(gr, gr, zero), zero);
+      const float2 mf = split(m[h][k]), vf = split(v[h][k]);
+      float2 w = split(pair_of<T, 4>(pv[h], k));
+      if (MASTER) {
+        w.x = same(from_f32<T>(ms[h][2 * k]), pv[h].e[2 * k]) ? ms[h][2 * k] : w.x;
+        w.y = same(from_f32<T>(ms[h][2 * k + 1]), pv[h].e[2 * k + 1]) ? ms[h][2 * k + 1] : w.y;
+      }
+      w.x = changed(w.x, mf.x, vf.x, hy, nu);
+      w.y = changed(w.y, mf.y, vf.y, hy, nu);
+      if (MASTER) {
+        ms[h][2 * k] = FULL || at + h * 128 + lane4 + 2 * k < n ? w.x : 0.0f;
+        ms[h][2 * k + 1] = FULL || at + h * 128 + lane4 + 2 * k + 1 < n ? w.y : 0.0f;
+      }
+      set_pair<T, 4>(pv[h], k, two(w.x, w.y));
+    }
+    if (FULL) store_vec<T, 4>(p + h * 128, pv[h]);
+    else store4(p, at + h * 128 + lane4, n, vec, pv[h]);
+    if (MASTER) wp[32 * h] = *reinterpret_cast<const float4*>(ms[h]);
+  }
+  if (BITS == 8) {
+    unsigned m_most, v_most;
+    bool finite;
+    block_sizes(m, v, m_most, v_most, finite);
+    const float tiny = __int_as_float(1 << 23);         // the smallest normal: its reciprocal is finite
+    m_unit = fmaxf(__uint_as_float(m_most) * (1.0f / 448.0f), tiny);
+    v_unit = fmaxf(__uint_as_float(v_most) * (1.0f / 57344.0f), tiny);
+    if (lane4 == 0) {
+      fl.m_scale[flat / QBLOCK] = m_unit;
+      fl.v_scale[flat / QBLOCK] = v_unit;
+    }
+    const Two mu = two(-m_unit), vu = two(-v_unit), mi = two(1.0f / m_unit), vi = two(1.0f / v_unit);
+    uint32_t* mp = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(fl.m) + flat + lane4);
+    uint32_t* vp = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(fl.v) + flat + lane4);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint64_t first = nu.key + (uint64_t)((flat + h * 128 + lane4) >> 1);
+      uint32_t mc = 0, vc = 0;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const uint64_t word = mix64(first + k);
+        const unsigned lo = (unsigned)word, hi = (unsigned)(word >> 32);
+        const float2 mf = split(m[h][k]), vf = split(v[h][k]);
+        const float2 mq = split(quotient_rz(two(fabsf(mf.x), fabsf(mf.y)), mu, mi)), vq = split(quotient_rz(v[h][k], vu, vi));
+        float2 a = make_float2(copysignf(round_carry<3, -6>(mq.x, lo & 0xffff), mf.x),
+                               copysignf(round_carry<3, -6>(mq.y, hi & 0xffff), mf.y));
+        float2 b = make_float2(round_carry<2, -14>(vq.x, lo >> 16), round_carry<2, -14>(vq.y, hi >> 16));
+        const float least = 1.52587890625e-05f;                         // 2^-16, the smallest code above zero
+        if (vf.x > 0.0f) b.x = fmaxf(b.x, least);
+        if (vf.y > 0.0f) b.y = fmaxf(b.y, least);
+        if (!finite) {
+          const float nan = __int_as_float(0x7fffffff);
+          if ((__float_as_uint(mf.x) & 0x7fffffffu) >= INF_BITS) a.x = nan;
+          if ((__float_as_uint(mf.y) & 0x7fffffffu) >= INF_BITS) a.y = nan;
+          if ((__float_as_uint(vf.x) & 0x7fffffffu) >= INF_BITS) b.x = nan;
+          if ((__float_as_uint(vf.y) & 0x7fffffffu) >= INF_BITS) b.y = nan;
+        }
+        mc |= (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) << (16 * k);
+        vc |= (uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E5M2) << (16 * k);
+      }
+      mp[32 * h] = mc;
+      vp[32 * h] = vc;
+    }
+  } else {
+    float4* mp = reinterpret_cast<float4*>(reinterpret_cast<float*>(fl.m) + flat + lane4);
+    float4* vp = reinterpret_cast<float4*>(reinterpret_cast<float*>(fl.v) + flat + lane4);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const float2 a = split(m[h][0]), b = split(m[h][1]), c = split(v[h][0]), d = split(v[h][1]);
+      mp[32 * h] = make_float4(a.x, a.y, b.x, b.y);
+      vp[32 * h] = make_float4(c.x, c.y, d.x, d.y);
+    }
+  }
+}
 
 template <typename T, int N, int BITS, bool MASTER>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, blocks_per_sm(BITS))
     k_adamw(const __grid_constant__ Table<N> tab, const __grid_constant__ Hyper hy, const __grid_constant__ Flat fl) {
   __shared__ double s[THREADS / 32];
   const int64_t pieces = tab.first[tab.count];
-  float clip = 1.0f;
+  Numbers nu = {1.0f, 0.0f, 0.0f, 0};
   if (fl.partial) {
     double sum = 0.0;
     for (int i = threadIdx.x; i < fl.partials; i += THREADS) sum += fl.partial[i];
     const double norm = sqrt(block_sum(sum, s));
     const double c = hy.max_norm / (norm + 1e-6);
-    clip = c < 1.0 || c != c ? (float)c : 1.0f;
+    nu.clip = c < 1.0 || c != c ? (float)c : 1.0f;
     if (blockIdx.x == 0 && threadIdx.x == 0 && fl.norm) *fl.norm = (float)norm;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t step = -1;
-  float rate = 0.0f, root = 0.0f;
-  uint64_t key = 0;
   for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
     const int i = tensor_of(tab, piece);
-    const int64_t n = tab.t[i].n, at = (piece - tab.first[i]) * PIECE + warp * QBLOCK;
+    const int64_t n = tab.t[i].n, at = (piece - tab.first[i]) * PIECE + (threadIdx.x >> 5) * QBLOCK;
     T* p = reinterpret_cast<T*>(tab.t[i].p);
     const T* g = reinterpret_cast<const T*>(tab.t[i].g);
     const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(T) - 1)) == 0;
@@ -235,135 +412,13 @@ __global__ void __launch_bounds__(THREADS)
         x1 *= x1;
         x2 *= x2;
       }
-      rate = (float)(hy.lr / (1.0 - p1));
-      root = (float)(1.0 / sqrt(1.0 - p2));
-      key = mix64(fl.seed ^ mix64((uint64_t)t));
+      nu.rate = (float)(hy.lr / (1.0 - p1));
+      nu.root = (float)(1.0 / sqrt(1.0 - p2));
+      nu.key = mix64(fl.seed ^ mix64((uint64_t)t));
     }
     if (at >= n) continue;                         // the warp's part lies past the tensor's end
-    Vec<T, 4> pv[2], gv[2];
-    float m[2][4], v[2][4], ms[2][4];
-    float m_unit = 0.0f, v_unit = 0.0f;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int64_t e = at + h * 128 + lane * 4;
-      pv[h] = load4(p, e, n, vec);
-      gv[h] = load4(g, e, n, vec);
-    }
-    if (BITS == 8) {
-      m_unit = fl.m_scale[flat / QBLOCK];
-      v_unit = fl.v_scale[flat / QBLOCK];
-    }
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int64_t f = flat + h * 128 + lane * 4;
-      if (BITS == 8) {
-        const uint32_t mc = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(fl.m) + f);
-        const uint32_t vc = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(fl.v) + f);
-        const float2 m0 = unpack8(mc & 0xffff, __NV_E4M3), m1 = unpack8(mc >> 16, __NV_E4M3);
-        const float2 v0 = unpack8(vc & 0xffff, __NV_E5M2), v1 = unpack8(vc >> 16, __NV_E5M2);
-        m[h][0] = m0.x * m_unit; m[h][1] = m0.y * m_unit; m[h][2] = m1.x * m_unit; m[h][3] = m1.y * m_unit;
-        v[h][0] = v0.x * v_unit; v[h][1] = v0.y * v_unit; v[h][2] = v1.x * v_unit; v[h][3] = v1.y * v_unit;
-      } else {
-        const float4 mf = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(fl.m) + f);
-        const float4 vf = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(fl.v) + f);
-        m[h][0] = mf.x; m[h][1] = mf.y; m[h][2] = mf.z; m[h][3] = mf.w;
-        v[h][0] = vf.x; v[h][1] = vf.y; v[h][2] = vf.z; v[h][3] = vf.w;
-      }
-      if (MASTER) {
-        const float4 w = *reinterpret_cast<const float4*>(fl.master + f);
-        ms[h][0] = w.x; ms[h][1] = w.y; ms[h][2] = w.z; ms[h][3] = w.w;
-      }
-    }
-    // past the tensor's end the gradient and the moments are zero, and stay it
-    float m_most = 0.0f, v_most = 0.0f;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int64_t e = at + h * 128 + lane * 4;
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float gr = to_f32(gv[h].e[k]) * clip;
-        // each product rounded by itself, as torch's expressions do
-        m[h][k] = __fadd_rn(__fmul_rn(hy.keep1, m[h][k]), __fmul_rn(hy.new1, gr));
-        v[h][k] = __fadd_rn(__fmul_rn(hy.keep2, v[h][k]), __fmul_rn(hy.new2, __fmul_rn(gr, gr)));
-        float w = to_f32(pv[h].e[k]);
-        if (MASTER) {
-          Vec<T, 1> rounded, now;
-          rounded.e[0] = from_f32<T>(ms[h][k]);
-          now.e[0] = pv[h].e[k];
-          w = rounded.r == now.r ? ms[h][k] : w;
-        }
-        // the change is good to some 2^-21 of itself (approximate root and quotient): far below the
-        // parameter's rounding
-        w = fmaf(w, hy.decay, -__fdividef(rate * m[h][k], fmaf(root_of(v[h][k]), root, hy.eps)));
-        if (MASTER) ms[h][k] = w;
-        pv[h].e[k] = from_f32<T>(w);
-        if (BITS == 8) {
-          m_most = fmaxf(m_most, fabsf(m[h][k]));         // a NaN does not count
-          v_most = fmaxf(v_most, v[h][k]);
-        }
-      }
-      store4(p, e, n, vec, pv[h]);
-    }
-    float mi = 0.0f, vi = 0.0f;
-    if (BITS == 8) {
-      const float tiny = __int_as_float(1 << 23);       // the smallest normal: its reciprocal is finite
-      m_most = warp_max(m_most);
-      v_most = warp_max(v_most);
-      if (!(m_most < INF) || !(v_most < INF)) {         // an infinity somewhere: the largest finite ones
-        m_most = v_most = 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            m_most = fmaxf(m_most, fabsf(m[h][k]) < INF ? fabsf(m[h][k]) : 0.0f);
-            v_most = fmaxf(v_most, v[h][k] < INF ? v[h][k] : 0.0f);
-          }
-        m_most = warp_max(m_most);
-        v_most = warp_max(v_most);
-      }
-      m_unit = fmaxf(m_most * (1.0f / 448.0f), tiny);
-      v_unit = fmaxf(v_most * (1.0f / 57344.0f), tiny);
-      if (lane == 0) {
-        fl.m_scale[flat / QBLOCK] = m_unit;
-        fl.v_scale[flat / QBLOCK] = v_unit;
-      }
-      mi = 1.0f / m_unit;
-      vi = 1.0f / v_unit;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int64_t e = at + h * 128 + lane * 4, f = flat + h * 128 + lane * 4;
-      if (e >= n) continue;
-      if (BITS == 8) {
-        const uint64_t word0 = mix64(key + (uint64_t)(f >> 1)), word1 = mix64(key + (uint64_t)(f >> 1) + 1);
-        float mq[4], vq[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const unsigned bits = (unsigned)((k < 2 ? word0 : word1) >> (32 * (k & 1)));
-          const float a = fabsf(m[h][k]), b = v[h][k];
-          const float x = round_carry<3, -6>(quotient_rz(a, m_unit, mi), bits & 0xffff, 448.0f);
-          const float y = round_carry<2, -14>(quotient_rz(b, v_unit, vi), bits >> 16, 57344.0f);
-          mq[k] = a < INF ? copysignf(x, m[h][k]) : NOT_A_NUMBER;
-          // 2^-16, the smallest code, for what is above zero
-          vq[k] = b < INF ? (b > 0.0f ? fmaxf(y, 1.52587890625e-05f) : 0.0f) : NOT_A_NUMBER;
-        }
-        const uint32_t mc = __nv_cvt_float2_to_fp8x2(make_float2(mq[0], mq[1]), __NV_SATFINITE, __NV_E4M3) |
-                            (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(mq[2], mq[3]), __NV_SATFINITE, __NV_E4M3) << 16;
-        const uint32_t vc = __nv_cvt_float2_to_fp8x2(make_float2(vq[0], vq[1]), __NV_SATFINITE, __NV_E5M2) |
-                            (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(vq[2], vq[3]), __NV_SATFINITE, __NV_E5M2) << 16;
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(fl.m) + f) = mc;
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(fl.v) + f) = vc;
-      } else {
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(fl.m) + f) = make_float4(m[h][0], m[h][1], m[h][2], m[h][3]);
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(fl.v) + f) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
-      }
-      if (MASTER) {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (e + k >= n) ms[h][k] = 0.0f;
-        *reinterpret_cast<float4*>(fl.master + f) = make_float4(ms[h][0], ms[h][1], ms[h][2], ms[h][3]);
-      }
-    }
+    if (vec && at + QBLOCK <= n) update_block<T, BITS, MASTER, true>(p, g, n, at, flat, vec, hy, fl, nu);
+    else update_block<T, BITS, MASTER, false>(p, g, n, at, flat, vec, hy, fl, nu);
   }
   // every block has read its counts before its ticket; the last one to take one raises them
   __shared__ bool last;
@@ -377,10 +432,6 @@ __global__ void __launch_bounds__(THREADS)
     for (int i = threadIdx.x; i < tab.count; i += THREADS) fl.steps[tab.index[i]] += 1;
 }
 
-constexpr int BLOCKS_PER_SM = 4;
-
-#undef INF
-#undef NOT_A_NUMBER
 
 template <int N>
 void fill(Table<N>& tab, int piece, int count, void* const* p, const void* const* g, const int64_t* n, const int64_t* at,
@@ -396,8 +447,8 @@ void fill(Table<N>& tab, int piece, int count, void* const* p, const void* const
   tab.count = count;
 }
 
-inline unsigned blocks_for(int64_t pieces) {
-  const int64_t most = (int64_t)sm_count() * BLOCKS_PER_SM;
+inline unsigned blocks_for(int64_t pieces, int per_sm) {
+  const int64_t most = (int64_t)sm_count() * per_sm;
   return (unsigned)(pieces < most ? pieces : most);
 }
 
@@ -405,7 +456,7 @@ template <typename T, int N>
 int squares(int count, const void* const* g, const int64_t* n, double* partial, int room, int* used, cudaStream_t st) {
   Table<N> tab;
   fill<N>(tab, NORM_PIECE, count, nullptr, g, n, nullptr, nullptr);
-  unsigned grid = blocks_for(tab.first[count]);
+  unsigned grid = blocks_for(tab.first[count], NORM_BLOCKS_PER_SM);
   if ((int)grid > room) grid = room;
   k_grad_squares<T, N><<<grid, THREADS, 0, st>>>(tab, partial);
   *used = (int)grid;
@@ -417,7 +468,7 @@ int update(int count, void* const* p, const void* const* g, const int64_t* n, co
            const Hyper& hy, const Flat& fl, int bits, cudaStream_t st) {
   Table<N> tab;
   fill<N>(tab, PIECE, count, p, g, n, at, index);
-  const unsigned grid = blocks_for(tab.first[count]);
+  const unsigned grid = blocks_for(tab.first[count], blocks_per_sm(bits));
   const auto go = [&](auto k) { k<<<grid, THREADS, 0, st>>>(tab, hy, fl); };
   if constexpr (sizeof(T) == 4) {
     bits == 8 ? go(k_adamw<T, N, 8, false>) : go(k_adamw<T, N, 32, false>);
@@ -483,6 +534,7 @@ extern "C" int f16_adamw_step(const f16_adamw_args* a, f16_stream_t stream) {
   hy.b2 = a->beta2;
   hy.eps = (float)a->eps;
   hy.decay = (float)(1.0 - a->lr * a->weight_decay);
+  hy.minus_zero = -0.0f;
   hy.keep1 = (float)a->beta1;
   hy.new1 = (float)(1.0 - a->beta1);
   hy.keep2 = (float)a->beta2;
