@@ -74,7 +74,7 @@ class ScanArgs(C.Structure):
                 ("hn", C.c_void_p), ("saved", C.c_void_p), ("dh", C.c_void_p), ("dh_t", C.c_int64),
                 ("dh_b", C.c_int64), ("dhn", C.c_void_p), ("dgate", C.c_void_p), ("dgate_t", C.c_int64),
                 ("dgate_b", C.c_int64), ("dx", C.c_void_p), ("dx_t", C.c_int64), ("dx_b", C.c_int64),
-                ("dh0", C.c_void_p)]
+                ("dh0", C.c_void_p), ("scratch", C.c_void_p), ("scratch_floats", C.c_int64)]
 
 
 class AdamwArgs(C.Structure):
@@ -141,6 +141,7 @@ _SIGS = {
                             _I64, _P], C.c_int),
     "f16_layer_norm_scratch_floats": ([_I64, C.c_int], _I64),
     "f16_scan_saved_floats": ([_I64, _I64, _I64], _I64),
+    "f16_scan_scratch_floats": ([_I64, _I64, _I64], _I64),
     "f16_scan_fwd": ([C.POINTER(ScanArgs), _P], C.c_int),
     "f16_scan_bwd": ([C.POINTER(ScanArgs), _P], C.c_int),
     "f16_scan_step": ([_P, _I64, _P, _I64, _I64, _I64, C.c_int, C.c_int, _P, C.c_int, _I64, _P, _I64, _P, _I64, _P],

@@ -28,8 +28,8 @@ namespace f16 {
 namespace opt {
 
 constexpr int THREADS = 256;
-// Resident update blocks, each walking over its share: 64 registers a thread, 80 for 8-bit moments.
-__host__ __device__ constexpr int blocks_per_sm(int bits) { return bits == 8 ? 3 : 4; }
+// Resident update blocks, each walking over its share: 64 registers a thread (80 and three blocks: +4% with 8-bit moments).
+constexpr int BLOCKS_PER_SM = 4;
 constexpr int NORM_BLOCKS_PER_SM = 4;
 constexpr int QBLOCK = F16_ADAMW_BLOCK;       // values of one scale: a warp's, 8 each
 constexpr int PIECE = THREADS / 32 * QBLOCK;  // values of a block at a time
@@ -378,7 +378,7 @@ __device__ __forceinline__ void update_block(T* p, const T* g, int64_t n, int64_
 }
 
 template <typename T, int N, int BITS, bool MASTER>
-__global__ void __launch_bounds__(THREADS, blocks_per_sm(BITS))
+__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM)
     k_adamw(const __grid_constant__ Table<N> tab, const __grid_constant__ Hyper hy, const __grid_constant__ Flat fl) {
   __shared__ double s[THREADS / 32];
   const int64_t pieces = tab.first[tab.count];
@@ -468,7 +468,7 @@ int update(int count, void* const* p, const void* const* g, const int64_t* n, co
            const Hyper& hy, const Flat& fl, int bits, cudaStream_t st) {
   Table<N> tab;
   fill<N>(tab, PIECE, count, p, g, n, at, index);
-  const unsigned grid = blocks_for(tab.first[count], blocks_per_sm(bits));
+  const unsigned grid = blocks_for(tab.first[count], BLOCKS_PER_SM);
   const auto go = [&](auto k) { k<<<grid, THREADS, 0, st>>>(tab, hy, fl); };
   if constexpr (sizeof(T) == 4) {
     bits == 8 ? go(k_adamw<T, N, 8, false>) : go(k_adamw<T, N, 32, false>);

@@ -16,71 +16,116 @@
 //
 // A thread owns the V channels of 4 bytes (two 16-bit values, or one where rows are not aligned for
 // that), a warp 32 neighbours of them, and takes CHUNK steps at a time into registers.
-//  * Many channels (k_scan<SPLIT = false>): a warp walks through time alone, the state in registers.
-//  * Few (SPLIT = true): the warps of a block, and the blocks of a cluster, take consecutive chunks of
-//    the same channels.  A chunk maps the state before it to A h + B; the (A, B) of a block's warps
-//    meet in shared memory, those of the cluster's blocks in every block's shared memory (DSMEM), each
-//    warp folds those before it into its own first state and repeats its chunk from registers.  Data
-//    is read once, the order of all sums is fixed, and the blocks of a cluster are resident together,
-//    so nothing spins on memory.
-// A chunk that a reset cuts passes nothing of the state before it on.  That is kept as A = NaN, a
+//  * Many channels: a warp walks through time alone, the state in registers (k_scan, k_scan_grad).
+//  * Few: time is cut into segments as well, enough of them to fill the GPU.  A segment maps the state
+//    before it to A h + B; k_scan_fold makes (A, B) of every segment, k_scan_starts the states between them,
+//    and then the same kernels walk through all segments at once.  That reads the coefficients and one
+//    more input a second time (what L2 still holds of them from there: the walk begins at the end where the
+//    fold stopped), but no block waits for another, and the order of all sums is fixed.
+// A segment that a reset cuts passes nothing of the state before it on.  That is kept as A = NaN, a
 // selection (never a product with 0), so that an infinity or NaN left by the episode before does not
 // leak: a coefficient that is NaN itself makes B NaN as well, so the two cannot be confused.
-#include <cooperative_groups.h>
-#include <type_traits>
 #include "typed.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace f16 {
 namespace scan {
 
 constexpr int CHUNK = F16_SCAN_CHUNK;     // steps in registers at a time, between saved states
-constexpr int MAX_WARPS = 16;             // of a block on consecutive chunks
-constexpr int MAX_CLUSTER = 8;            // blocks of a cluster on consecutive chunks
-constexpr int WIDE_WARPS = 4;             // of a block whose warps have channels of their own
-constexpr int WIDE_BLOCKS = 5, WIDE_GRAD_BLOCKS = 3;      // of those on an SM: 96 and 168 registers a thread
+constexpr int WARPS = 4;                  // of a block, each with channels (and a segment) of its own
+// Blocks on an SM: 96, 128 and 80 registers a thread.
+constexpr int WALK_BLOCKS = 5, GRAD_BLOCKS = 4, FOLD_BLOCKS = 6;
+constexpr int MAX_SEGMENT = F16_SCAN_SEGMENT;      // steps whose coefficients' product is formed
+constexpr int WARPS_PER_SM = 64;          // in all: with less than half of them, time is cut
 static_assert(CHUNK <= 32, "resets of a chunk are bits of one word");
 
 typedef f16_scan_args Args;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// V channels of a lane as one value: a float, or a pair computed with by one instruction.
+template <int V> struct Lanes { typedef float type; };
+template <> struct Lanes<2> { typedef Two type; };
+
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float less(float a, float b) { return a - b; }
+__device__ __forceinline__ Two less(Two a, Two b) { return fma2(b, two(-1.0f), a); }
+__device__ __forceinline__ float part(float v, int) { return v; }
+__device__ __forceinline__ float part(Two v, int k) {
+  const float2 f = split(v);
+  return k ? f.y : f.x;
 }
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ void join(float& v, float x, float) { v = x; }
+__device__ __forceinline__ void join(Two& v, float x, float y) { v = two(x, y); }
+template <typename P> __device__ __forceinline__ P all_of(float x);
+template <> __device__ __forceinline__ float all_of<float>(float x) { return x; }
+template <> __device__ __forceinline__ Two all_of<Two>(float x) { return two(x); }
+
+// The types' values as fp32 and back.
+template <typename T, int V>
+__device__ __forceinline__ typename Lanes<V>::type widen(const Vec<T, V>& v) {
+  if constexpr (V == 2) return pair_of<T, V>(v, 0);
+  else return to_f32(v.e[0]);
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(typename Lanes<V>::type f) {
+  Vec<T, V> v;
+  if constexpr (V == 2) set_pair<T, V>(v, 0, f);
+  else v.e[0] = from_f32<T>(f);
+  return v;
 }
 
-// A step's coefficients in one register.  Gated: the smaller one of f and 1 - f, e / (1 + e) with
-// e = exp(-|gate|), with the gate's sign: negative, it is f.  The other is its difference from 1, which
-// is at least 1/2 and so keeps every digit.  Raw: the coefficient itself.
-template <bool GATED>
-__device__ __forceinline__ float packed_gate(float g) {
-  if (!GATED) return g;
-  const float e = ex2(-1.4426950408889634f * fabsf(g));
-  return copysignf(e * rcp(1.0f + e), g);
+// f = sigmoid(g) and k = 1 - f: with e = exp(g), k = 1 / (1 + e) and f = e k, each good to a few units of
+// its own last place (neither is a difference).  exp(g) is held at 2^126 and below, where k is 2^-126.
+__device__ __forceinline__ float capped_exp2(float t) {
+  float e;
+  asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(e) : "f"(t));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(e));
+  return e;
 }
-template <bool GATED>
-__device__ __forceinline__ void coefficients(float s, float& a, float& k) {
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void sigmoid(float g, float& f, float& k) {
+  const float e = capped_exp2(g * 1.4426950408889634f);
+  k = reciprocal(1.0f + e);
+  f = e * k;
+}
+__device__ __forceinline__ void sigmoid(Two g, Two& f, Two& k) {
+  const float2 t = split(g * two(1.4426950408889634f));
+  const Two e = two(capped_exp2(t.x), capped_exp2(t.y));
+  const float2 d = split(e + two(1.0f));
+  k = two(reciprocal(d.x), reciprocal(d.y));
+  f = e * k;
+}
+
+// A step's coefficient a and inflow b; k: 1 - a (gated only).
+template <bool GATED, typename P>
+__device__ __forceinline__ void step_of(P g, P x, P& a, P& b, P& k) {
   if (GATED) {
-    const float small = fabsf(s), big = 1.0f - small;
-    const bool neg = __float_as_int(s) < 0;
-    a = neg ? small : big;
-    k = neg ? big : small;
+    sigmoid(g, a, k);
+    b = k * x;
   } else {
-    a = s;
-    k = 1.0f;
+    a = g;
+    b = x;
+    k = g;
   }
 }
 
+// How the work is cut: `groups` of 32 V channels, `segments` of `length` steps (a multiple of CHUNK).
+struct Shape {
+  int64_t groups;
+  int segments, length;
+  float2* maps;           // (A, B) of [segments][channels], or NULL: one segment
+  float* starts;          // the state (gradient) that enters [segments][channels]
+};
+
 // h -> A h + B, where A is not NaN (cut) and h not zero (so that an overflown A cannot make NaN of it).
-__device__ __forceinline__ float pass_through(float A, float B, float h) {
-  return A != A || h == 0.0f ? B : fmaf(A, h, B);
+__device__ __forceinline__ float pass_through(float2 m, float h) {
+  return m.x != m.x || h == 0.0f ? m.y : fmaf(m.x, h, m.y);
 }
+// First m, then n.
+__device__ __forceinline__ float2 then(float2 m, float2 n) { return make_float2(n.x * m.x, pass_through(n, m.y)); }
+__device__ __forceinline__ float cut_mark() { return __int_as_float(0x7fffffff); }
 
 struct Lane {
   int64_t b, d, c;      // sequence, feature, channel = b dim + d
@@ -113,50 +158,22 @@ __device__ __forceinline__ bool reset_at(const Args& p, int64_t b, int64_t t) {
                             : __ldg(reinterpret_cast<const float*>(p.reset) + i) != 0.0f;
 }
 
-// Bit i: step t0 + i (of the n from t0 on) resets the lane's sequence.  Called by whole warps: where a warp
-// has one sequence its lanes read a step each.
-__device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0, int n) {
+// Bit i of resets_of: step t0 + i (of the n from t0 on) resets the lane's sequence.  Called by whole warps:
+// where a warp has one sequence its lanes read a step each, ahead of the time it is wanted (reset_ahead).
+__device__ __forceinline__ bool reset_ahead(const Args& p, const Lane& l, int t0) {
+  const int lane = threadIdx.x & 31, m = l.len - t0 < CHUNK ? l.len - t0 : CHUNK;
+  return p.reset && l.together && t0 >= 0 && lane < m && reset_at(p, l.b, t0 + lane);
+}
+__device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0, int n, bool ahead) {
   if (!p.reset) return 0;
-  if (l.together) {
-    const int lane = threadIdx.x & 31, m = l.len - t0 < CHUNK ? l.len - t0 : CHUNK;
-    return __ballot_sync(~0u, t0 >= 0 && lane < m && reset_at(p, l.b, t0 + lane));
-  }
+  if (l.together) return __ballot_sync(~0u, ahead);
   unsigned m = 0;
 #pragma unroll 1
   for (int i = 0; i < n; i++) m |= (unsigned)reset_at(p, l.b, t0 + i) << i;
   return m;
 }
-
-template <typename T, int V>
-__device__ __forceinline__ void unpack(const Vec<T, V>& v, float (&f)[V]) {
-  if constexpr (sizeof(T) == 2 && V == 2) {
-    float2 two;
-    if constexpr (std::is_same<T, __half>::value) {
-      two = __half22float2(*reinterpret_cast<const __half2*>(&v));
-    } else {
-      two = make_float2(__uint_as_float(v.r << 16), __uint_as_float(v.r & 0xffff0000u));
-    }
-    f[0] = two.x;
-    f[1] = two.y;
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; k++) f[k] = to_f32(v.e[k]);
-  }
-}
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> pack(const float (&f)[V]) {
-  Vec<T, V> v;
-  if constexpr (std::is_same<T, __nv_bfloat16>::value && V == 2) {
-    const __nv_bfloat162 two = __floats2bfloat162_rn(f[0], f[1]);
-    v.r = *reinterpret_cast<const unsigned*>(&two);
-  } else if constexpr (std::is_same<T, __half>::value && V == 2) {
-    const __half2 two = __floats2half2_rn(f[0], f[1]);
-    v.r = *reinterpret_cast<const unsigned*>(&two);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; k++) v.e[k] = from_f32<T>(f[k]);
-  }
-  return v;
+__device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0, int n) {
+  return resets_of(p, l, t0, n, reset_ahead(p, l, t0));
 }
 
 // A tensor's element (t0, b, d), and how far it is to the next step's.
@@ -190,319 +207,356 @@ __device__ __forceinline__ void load_chunk(Vec<T, V> (&v)[CHUNK], const Line<T>&
 }
 
 template <int V>
-__device__ __forceinline__ void load_state(float (&h)[V], const float* p, const Lane& l) {
-#pragma unroll
-  for (int k = 0; k < V; k++) h[k] = p && l.live ? p[l.c + k] : 0.0f;
+__device__ __forceinline__ typename Lanes<V>::type load_state(const float* p, const Lane& l) {
+  typename Lanes<V>::type v;
+  const bool there = p && l.live;
+  join(v, there ? p[l.c] : 0.0f, there && V > 1 ? p[l.c + V - 1] : 0.0f);
+  return v;
 }
 template <int V>
-__device__ __forceinline__ void store_state(float* p, const float (&h)[V], const Lane& l) {
+__device__ __forceinline__ void store_state(float* p, typename Lanes<V>::type v, const Lane& l) {
   if (p && l.live) {
 #pragma unroll
-    for (int k = 0; k < V; k++) p[l.c + k] = h[k];
+    for (int k = 0; k < V; k++) p[l.c + k] = part(v, k);
   }
 }
-
-// What the warps of a block and the blocks of a cluster tell one another, twice (a tile's is still
-// read while the next one's is written).
-template <int V>
-struct Shared {
-  float2 warp[2][MAX_WARPS][32][V];
-  float2 block[2][MAX_CLUSTER][32][V];
-};
-
-// (A, B) of this warp's chunk in, the state before the chunk out; `carry`, the state before the tile,
-// becomes the state after it.
-template <int V>
-__device__ __forceinline__ void join(Shared<V>& s, int half, int warps, int blocks, int rank, const float (&A)[V],
-                                     const float (&B)[V], float (&carry)[V], float (&before)[V]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int k = 0; k < V; k++) s.warp[half][warp][lane][k] = make_float2(A[k], B[k]);
-  __syncthreads();
-  if (blocks > 1) {
-    // the block's own map, to block `warp` of the cluster: the first `blocks` warps each serve one
-    // (a tile of a cluster has as many warps as blocks at least)
-    if (warp < blocks) {
-      Shared<V>* there = cg::this_cluster().map_shared_rank(&s, warp);
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        float2 all = s.warp[half][0][lane][k];
-        for (int w = 1; w < warps; w++) {
-          const float2 m = s.warp[half][w][lane][k];
-          all.y = pass_through(m.x, m.y, all.y);
-          all.x = m.x * all.x;              // NaN (cut) stays NaN
-        }
-        there->block[half][rank][lane][k] = all;
-      }
-    }
-    cg::this_cluster().sync();
-  }
-#pragma unroll
-  for (int k = 0; k < V; k++) {
-    float h = carry[k], mine = h;
-    if (blocks > 1) {
-      for (int r = 0; r < blocks; r++) {
-        if (r == rank) mine = h;
-        const float2 m = s.block[half][r][lane][k];
-        h = pass_through(m.x, m.y, h);
-      }
-    }
-    float at = mine;
-    for (int w = 0; w < warps; w++) {
-      if (w == warp) before[k] = at;
-      if (w == warp && blocks > 1) break;
-      const float2 m = s.warp[half][w][lane][k];
-      at = pass_through(m.x, m.y, at);
-    }
-    carry[k] = blocks > 1 ? h : at;
-  }
+// Where `yes`, y instead of x.
+__device__ __forceinline__ float pick(bool yes, float y, float x) { return yes ? y : x; }
+__device__ __forceinline__ Two pick(bool yes, Two y, Two x) {
+  const float2 a = split(y), b = split(x);
+  return two(yes ? a.x : b.x, yes ? a.y : b.y);
 }
 
 // The steps of a chunk from the state h on, written to `out`.  PLAIN: every lane has all CHUNK steps and no
-// reset among them.  s: the packed coefficients (gated; raw ones are read from g).
-template <typename T, int V, bool GATED, bool PLAIN>
-__device__ __forceinline__ void walk(const Vec<T, V> (&g)[CHUNK], const float (&s)[GATED ? CHUNK : 1][V],
-                                     const Vec<T, V> (&x)[CHUNK], unsigned cut, int n, int left, bool live, Line<T> out,
-                                     float (&h)[V]) {
+// reset among them.
+template <typename T, int V, bool GATED, bool PLAIN, typename P>
+__device__ __forceinline__ void walk(const Vec<T, V> (&g)[CHUNK], const Vec<T, V> (&x)[CHUNK], unsigned cut, int n,
+                                     int left, bool live, Line<T> out, P& h) {
 #pragma unroll
   for (int i = 0; i < CHUNK; i++) {
-    float xf[V], gf[V], o[V];
-    unpack<T, V>(x[i], xf);
-    if (!GATED) unpack<T, V>(g[i], gf);
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-      float a, c;
-      coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
-      const float b = GATED ? c * xf[k] : xf[k];
-      if (PLAIN) {
-        h[k] = fmaf(a, h[k], b);
-        o[k] = h[k];
-      } else {
-        if (i < n) h[k] = cut >> i & 1 ? b : fmaf(a, h[k], b);
-        o[k] = i < n ? h[k] : 0.0f;
-      }
+    P a, b, k;
+    step_of<GATED>(widen(g[i]), widen(x[i]), a, b, k);
+    P o;
+    if (PLAIN) {
+      o = h = fma2(a, h, b);
+    } else {
+      h = pick(i < n, pick(cut >> i & 1, b, fma2(a, h, b)), h);
+      o = pick(i < n, h, all_of<P>(0.0f));
     }
-    if (PLAIN || (live && i < left)) store_vec<T, V>(out.p, pack<T, V>(o));
+    if (PLAIN || (live && i < left)) store_vec<T, V>(out.p, narrow<T, V>(o));
     advance(out.p, out.st);
   }
 }
 
+// The warp's segment and channels; false: there are none.  The last task first: see the file's head.
+__device__ __forceinline__ bool task_of(const Args& p, const Shape& sh, int v, bool last_first, int& segment, Lane& l) {
+  int64_t task = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  const int64_t tasks = sh.groups * sh.segments;
+  if (task >= tasks) return false;
+  if (last_first) task = tasks - 1 - task;
+  segment = (int)(task / sh.groups);
+  l = lane_of(p, ((task - segment * sh.groups) * 32 + (threadIdx.x & 31)) * v);
+  return true;
+}
+
+// How many of the CHUNK steps from t0 on the lane's sequence has.
+__device__ __forceinline__ int steps_of(const Lane& l, int t0) {
+  return l.live ? (l.len - t0 < CHUNK ? l.len - t0 : CHUNK) : 0;
+}
+
 template <typename T, int V, bool GATED>
-__device__ __forceinline__ void pack_gates(const Vec<T, V> (&g)[CHUNK], float (&s)[GATED ? CHUNK : 1][V]) {
-  if constexpr (GATED) {
+__global__ void __launch_bounds__(32 * WARPS, WALK_BLOCKS) k_scan(const __grid_constant__ Args p, const __grid_constant__ Shape sh) {
+  int segment;
+  Lane l;
+  if (!task_of(p, sh, V, sh.maps, segment, l)) return;
+  const int steps = (int)p.steps, begin = segment * sh.length;
+  const int end = steps - begin < sh.length ? steps : begin + sh.length;
+  const int64_t channels = p.batch * p.dim;
+  typename Lanes<V>::type h = load_state<V>(segment ? sh.starts + segment * channels : p.h0, l);
+  for (int t0 = begin; t0 < end; t0 += CHUNK) {
+    const int n = steps_of(l, t0), left = steps - t0;
+    const bool all = __all_sync(~0u, n == CHUNK);
+    Vec<T, V> g[CHUNK], x[CHUNK];
+    load_chunk<T, V>(g, Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
+    load_chunk<T, V>(x, Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
+    const unsigned cut = resets_of(p, l, t0, n);
+    const bool plain = all && __all_sync(~0u, cut == 0);
+    if (p.saved) store_state<V>(p.saved + (int64_t)(t0 / CHUNK) * channels, h, l);
+    const Line<T> out(p.h, p.h_t, p.h_b, l, t0);
+    if (plain) walk<T, V, GATED, true>(g, x, 0, CHUNK, CHUNK, true, out, h);
+    else walk<T, V, GATED, false>(g, x, cut, n, left, l.live, out, h);
+  }
+  if (end == steps) store_state<V>(p.hn, h, l);
+}
+
+// A chunk's steps folded into (A, B).
+template <typename T, int V, bool GATED, bool BACK, bool PLAIN, typename P>
+__device__ __forceinline__ void fold(const Vec<T, V> (&g)[CHUNK], const Vec<T, V> (&x)[CHUNK], unsigned cut, int n, P& A, P& B) {
 #pragma unroll
-    for (int i = 0; i < CHUNK; i++) {
-      float gf[V];
-      unpack<T, V>(g[i], gf);
-#pragma unroll
-      for (int k = 0; k < V; k++) s[i][k] = packed_gate<true>(gf[k]);
+  for (int j = 0; j < CHUNK; j++) {
+    const int i = BACK ? CHUNK - 1 - j : j;
+    P a, b, k;
+    step_of<GATED>(widen(g[i]), widen(x[i]), a, b, k);
+    const P nextA = A * a, nextB = BACK ? a * (widen(x[i]) + B) : fma2(a, B, b);
+    if (PLAIN) {
+      A = nextA;
+      B = nextB;
+    } else {
+      const bool r = cut >> i & 1;
+      A = pick(i < n, pick(r, all_of<P>(cut_mark()), nextA), A);
+      B = pick(i < n, pick(r, BACK ? all_of<P>(0.0f) : b, nextB), B);
     }
   }
 }
 
-template <typename T, int V, bool GATED, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS, SPLIT ? 1 : WIDE_BLOCKS)
-    k_scan(const __grid_constant__ Args p, int blocks) {
-  const int warp = threadIdx.x >> 5, warps = SPLIT ? blockDim.x >> 5 : 1;
-  const int rank = SPLIT ? (int)(blockIdx.x % blocks) : 0;
-  const int64_t group = SPLIT ? blockIdx.x / blocks : (int64_t)blockIdx.x * WIDE_WARPS + warp;
-  const Lane l = lane_of(p, (group * 32 + (threadIdx.x & 31)) * V);
-  const int tile = CHUNK * (SPLIT ? warps * blocks : 1), T_ = (int)p.steps;
-  float h[V];
-  load_state<V>(h, p.h0, l);
-  if (SPLIT && blocks > 1) cg::this_cluster().sync();      // every block has begun
-  const int mine = SPLIT ? (rank * warps + warp) * CHUNK : 0;
-  const auto steps_at = [&](int t0) { return l.live ? (l.len - t0 < CHUNK ? l.len - t0 : CHUNK) : 0; };
-  Vec<T, V> g[CHUNK], x[CHUNK];
-  const auto fetch = [&](int t0) {
-    const int n = steps_at(t0);
+// (A, B) of the warp's segment: of the states, or (BACK) of their gradients in reverse time, where B gathers
+// what the segment's own dh send to the state before it.
+template <typename T, int V, bool GATED, bool BACK>
+__global__ void __launch_bounds__(32 * WARPS, FOLD_BLOCKS)
+    k_scan_fold(const __grid_constant__ Args p, const __grid_constant__ Shape sh) {
+  int segment;
+  Lane l;
+  if (!task_of(p, sh, V, false, segment, l)) return;
+  const int steps = (int)p.steps, begin = segment * sh.length;
+  const int end = steps - begin < sh.length ? steps : begin + sh.length;
+  const int chunks = (end - begin + CHUNK - 1) / CHUNK;
+  typedef typename Lanes<V>::type P;
+  P A = all_of<P>(1.0f), B = all_of<P>(0.0f);
+  for (int c = 0; c < chunks; c++) {
+    const int t0 = begin + (BACK ? chunks - 1 - c : c) * CHUNK, n = steps_of(l, t0);
     const bool all = __all_sync(~0u, n == CHUNK);
+    Vec<T, V> g[CHUNK], x[CHUNK];
     load_chunk<T, V>(g, Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
-    load_chunk<T, V>(x, Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
-    return resets_of(p, l, t0, n);
-  };
-  int half = 0;
-  for (int base = 0; base < T_; base += tile, half ^= 1) {
-    const int t0 = base + mine, left = T_ - t0, n = steps_at(t0);
-    const unsigned cut = fetch(t0);
-    const bool plain = __all_sync(~0u, n == CHUNK && cut == 0);
-    float s[GATED ? CHUNK : 1][V];
-    pack_gates<T, V, GATED>(g, s);
-    float before[V];
-    if (SPLIT) {
-      __shared__ Shared<V> sh;
-      float A[V], B[V];
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        A[k] = 1.0f;
-        B[k] = 0.0f;
-      }
-#pragma unroll
-      for (int i = 0; i < CHUNK; i++) {
-        float xf[V], gf[V];
-        unpack<T, V>(x[i], xf);
-        if (!GATED) unpack<T, V>(g[i], gf);
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-          float a, c;
-          coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
-          const float b = GATED ? c * xf[k] : xf[k];
-          if (i < n) {
-            const bool r = cut >> i & 1;
-            A[k] = r ? __int_as_float(0x7fffffff) : A[k] * a;
-            B[k] = r ? b : fmaf(a, B[k], b);
-          }
-        }
-      }
-      join<V>(sh, half, warps, blocks, rank, A, B, h, before);
-      // h is the state after the tile now; the chunk is repeated from `before`
+    if (!BACK || p.dh) {
+      load_chunk<T, V>(x, BACK ? Line<T>(p.dh, p.dh_t, p.dh_b, l, t0) : Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
     } else {
 #pragma unroll
-      for (int k = 0; k < V; k++) before[k] = h[k];
+      for (int i = 0; i < CHUNK; i++) x[i] = narrow<T, V>(all_of<P>(0.0f));
     }
-    if (p.saved && left > 0) store_state<V>(p.saved + (int64_t)(t0 / CHUNK) * p.batch * p.dim, before, l);
-    const Line<T> out(p.h, p.h_t, p.h_b, l, t0);
-    if (plain) walk<T, V, GATED, true>(g, s, x, 0, CHUNK, CHUNK, true, out, before);
-    else walk<T, V, GATED, false>(g, s, x, cut, n, left, l.live, out, before);
-    if (!SPLIT) {
+    const unsigned cut = resets_of(p, l, t0, n);
+    if (all && __all_sync(~0u, cut == 0)) fold<T, V, GATED, BACK, true>(g, x, 0, CHUNK, A, B);
+    else fold<T, V, GATED, BACK, false>(g, x, cut, n, A, B);
+  }
+  if (l.live) {
+    float2* out = sh.maps + segment * (p.batch * p.dim) + l.c;
 #pragma unroll
-      for (int k = 0; k < V; k++) h[k] = before[k];
+    for (int k = 0; k < V; k++) out[k] = make_float2(part(A, k), part(B, k));
+  }
+}
+
+// What enters each segment, from the first on (BACK: the last): the maps of the segments before it, folded in
+// order.  32 channels a block, a warp on consecutive segments; `first`: what enters the first one, or NULL.
+constexpr int START_WARPS = 32, START_EACH = 16;      // warps of a block, segments of a warp at a time
+template <bool BACK>
+__global__ void __launch_bounds__(32 * START_WARPS) k_scan_starts(const __grid_constant__ Shape sh, int64_t channels, const float* first) {
+  __shared__ float2 of_warp[START_WARPS][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const bool live = c < channels;
+  float h = first && live ? first[c] : 0.0f;
+  for (int base = 0; base < sh.segments; base += START_WARPS * START_EACH) {
+    const int begin = base + warp * START_EACH;
+    const auto at = [&](int i) { return (BACK ? sh.segments - 1 - i : i) * channels + c; };
+    float2 m[START_EACH], all = make_float2(1.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < START_EACH; i++) m[i] = live && begin + i < sh.segments ? sh.maps[at(begin + i)] : make_float2(1.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < START_EACH; i++) all = then(all, m[i]);
+    of_warp[warp][lane] = all;
+    __syncthreads();
+    float mine = h;
+#pragma unroll 8
+    for (int w = 0; w < START_WARPS; w++) {
+      if (w == warp) mine = h;
+      h = pass_through(of_warp[w][lane], h);
+    }
+#pragma unroll
+    for (int i = 0; i < START_EACH; i++) {
+      if (live && begin + i < sh.segments) sh.starts[at(begin + i)] = mine;
+      mine = pass_through(m[i], mine);
+    }
+    __syncthreads();
+  }
+}
+
+// A chunk of the backward pass's three inputs, as the lane's own values: in shared memory, where the copies of
+// the next chunk land while this one is worked on (4-byte lanes), or in registers.
+constexpr int STAGES = 2;
+template <typename T, int V, bool STAGED> struct Inputs;
+template <typename T, int V> struct Inputs<T, V, true> {
+  typedef unsigned Buffer[STAGES][3][CHUNK][32 * WARPS];
+  unsigned* mine;
+  bool with_dh, rows;           // rows: a warp's row is 128 aligned bytes of one sequence in all three
+  __device__ __forceinline__ Inputs(Buffer& b, const Args& p, const Lane& l) : mine(&b[0][0][0][threadIdx.x]), with_dh(p.dh) {
+    const auto whole = [&](const void* q, int64_t st, int64_t sb) {
+      return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ((st | sb) & (4 * V - 1)) == 0;
+    };
+    rows = l.together && __all_sync(~0u, l.live) && p.dim % (4 * V) == 0 && whole(p.gate, p.gate_t, p.gate_b) &&
+           whole(p.x, p.x_t, p.x_b) && (!with_dh || whole(p.dh, p.dh_t, p.dh_b));
+  }
+  __device__ __forceinline__ unsigned* at(int stage, int which, int i) const {
+    return mine + ((stage * 3 + which) * CHUNK + i) * 32 * WARPS;
+  }
+  __device__ __forceinline__ Vec<T, V> get(int stage, int which, int i) const {
+    Vec<T, V> v;
+    v.r = *at(stage, which, i);
+    return v;
+  }
+  __device__ __forceinline__ Vec<T, V> gate(int stage, int i) const { return get(stage, 0, i); }
+  __device__ __forceinline__ Vec<T, V> x(int stage, int i) const { return get(stage, 1, i); }
+  __device__ __forceinline__ typename Lanes<V>::type dh(int stage, int i) const {
+    return with_dh ? widen(get(stage, 2, i)) : all_of<typename Lanes<V>::type>(0.0f);
+  }
+  // Every lane its own 4 bytes.
+  __device__ __forceinline__ void copy(int stage, int which, Line<T> from, int n) {
+    unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, which, 0));
+#pragma unroll
+    for (int i = 0; i < CHUNK; i++) {
+      if (i < n) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + i * 128 * WARPS), "l"(from.p) : "memory");
+      advance(from.p, from.st);
     }
   }
-  if (!SPLIT || (rank == 0 && warp == 0)) store_state<V>(p.hn, h, l);
-}
+  // Eight lanes a row: 16 bytes each.
+  __device__ __forceinline__ void copy_rows(int stage, int which, const void* base, int64_t st, int64_t sb, const Lane& l,
+                                            int t0, int n) {
+    const int lane = threadIdx.x & 31, row = lane >> 3, col = lane & 7;
+    const T* from = reinterpret_cast<const T*>(base) + l.b * sb + (l.d - lane * V) + col * 4 * V + (int64_t)(t0 + row) * st;
+    unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, which, row) - lane + 4 * col);
+#pragma unroll
+    for (int i = 0; i < CHUNK / 4; i++) {
+      if (row + 4 * i < n) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * 4 * 128 * WARPS), "l"(from) : "memory");
+      advance(from, 4 * st);
+    }
+  }
+  __device__ __forceinline__ void fetch(const Args& p, const Lane& l, int stage, int t0, int n) {
+    if (rows) {
+      __syncwarp();             // every lane has read what this stage held
+      copy_rows(stage, 0, p.gate, p.gate_t, p.gate_b, l, t0, n);
+      copy_rows(stage, 1, p.x, p.x_t, p.x_b, l, t0, n);
+      if (with_dh) copy_rows(stage, 2, p.dh, p.dh_t, p.dh_b, l, t0, n);
+    } else {
+      const Line<T> g(p.gate, p.gate_t, p.gate_b, l, t0), x(p.x, p.x_t, p.x_b, l, t0), d(p.dh, p.dh_t, p.dh_b, l, t0);
+      copy(stage, 0, g, n);
+      copy(stage, 1, x, n);
+      if (with_dh) copy(stage, 2, d, n);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // The chunk fetched before the last one has landed, what the other lanes copied of it as well.
+  __device__ __forceinline__ void wait() {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (rows) __syncwarp();
+  }
+};
+template <typename T, int V> struct Inputs<T, V, false> {
+  typedef int Buffer;
+  Vec<T, V> in[STAGES][3][CHUNK];
+  bool with_dh;
+  __device__ __forceinline__ Inputs(Buffer&, const Args& p, const Lane&) : with_dh(p.dh) {}
+  __device__ __forceinline__ Vec<T, V> gate(int, int i) const { return in[0][0][i]; }
+  __device__ __forceinline__ Vec<T, V> x(int, int i) const { return in[0][1][i]; }
+  __device__ __forceinline__ typename Lanes<V>::type dh(int, int i) const {
+    return with_dh ? widen(in[0][2][i]) : all_of<typename Lanes<V>::type>(0.0f);
+  }
+  __device__ __forceinline__ void load(const Args& p, const Lane& l, int t0, int n) {
+    const bool all = __all_sync(~0u, n == CHUNK);
+    load_chunk<T, V>(in[0][0], Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
+    load_chunk<T, V>(in[0][1], Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
+    if (with_dh) load_chunk<T, V>(in[0][2], Line<T>(p.dh, p.dh_t, p.dh_b, l, t0), n, all);
+  }
+};
 
 // The steps of a chunk again from the saved state h, then their gradients from the last one back; carry: the
 // gradient that reaches the chunk's last state, then the one that leaves its first.
 // Gated: with d_t = f (h_{t-1} - x_t), dx_t = G k and dgate_t = dx_t d_t.
-template <typename T, int V, bool GATED, bool PLAIN>
-__device__ __forceinline__ void walk_back(const Vec<T, V> (&g)[CHUNK], const float (&s)[GATED ? CHUNK : 1][V],
-                                          const Vec<T, V> (&x)[CHUNK], const Vec<T, V> (&dh)[CHUNK], unsigned cut, int n,
-                                          int left, bool live, Line<T> dg, bool want_g, Line<T> dx, bool want_x,
-                                          float (&h)[V], float (&carry)[V]) {
-  float d[CHUNK][V];
+template <typename T, int V, bool GATED, bool PLAIN, typename I, typename P>
+__device__ __forceinline__ void walk_back(const I& in, int stage, unsigned cut, int n, int left, bool live,
+                                          Line<T> dg, bool want_g, Line<T> dx, bool want_x, P h, P& carry) {
+  const P zero = all_of<P>(0.0f);
+  P d[CHUNK];
 #pragma unroll
   for (int i = 0; i < CHUNK; i++) {
-    float xf[V], gf[V];
-    unpack<T, V>(x[i], xf);
-    if (!GATED) unpack<T, V>(g[i], gf);
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-      float a, c;
-      coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
-      const float b = GATED ? c * xf[k] : xf[k];
-      const bool r = !PLAIN && (cut >> i & 1);
-      const float hp = r ? 0.0f : h[k];
-      d[i][k] = GATED ? a * (hp - xf[k]) : hp;
-      h[k] = r ? b : fmaf(a, hp, b);
-    }
+    P a, b, k;
+    const P xf = widen(in.x(stage, i));
+    step_of<GATED>(widen(in.gate(stage, i)), xf, a, b, k);
+    const bool r = !PLAIN && (cut >> i & 1);
+    const P hp = PLAIN ? h : pick(r, zero, h);
+    d[i] = GATED ? a * less(hp, xf) : hp;
+    h = PLAIN ? fma2(a, hp, b) : pick(r, b, fma2(a, hp, b));
   }
+  asm volatile("" ::: "memory");        // the gates are read and worked out again, not kept
+  // what reaches a step's state from the step after it is pass * carry
+  P pass = all_of<P>(1.0f);
   const int last = CHUNK - 1;
   dg.p += last * dg.st;
   dx.p += last * dx.st;
 #pragma unroll
   for (int i = CHUNK - 1; i >= 0; i--) {
-    float gf[V], df[V], og[V], ox[V];
-    unpack<T, V>(dh[i], df);
-    if (!GATED) unpack<T, V>(g[i], gf);
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-      float a, c;
-      coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
-      const float G = df[k] + carry[k];
-      ox[k] = GATED ? G * c : G;
-      og[k] = ox[k] * d[i][k];
-      if (PLAIN) {
-        carry[k] = a * G;
-      } else {
-        if (i < n) carry[k] = cut >> i & 1 ? 0.0f : a * G;
-        if (i >= n) og[k] = ox[k] = 0.0f;
-      }
+    P a, b, k;
+    step_of<GATED>(widen(in.gate(stage, i)), zero, a, b, k);
+    const P G = fma2(pass, carry, in.dh(stage, i));
+    P ox = GATED ? G * k : G, og = ox * d[i];
+    if (PLAIN) {
+      pass = a;
+      carry = G;
+    } else {
+      const bool r = cut >> i & 1;
+      pass = pick(i < n, pick(r, zero, a), pass);
+      carry = pick(i < n, pick(r, zero, G), carry);
+      ox = pick(i < n, ox, zero);
+      og = pick(i < n, og, zero);
     }
     if (PLAIN || (live && i < left)) {
-      if (want_g) store_vec<T, V>(dg.p, pack<T, V>(og));
-      if (want_x) store_vec<T, V>(dx.p, pack<T, V>(ox));
+      if (want_g) store_vec<T, V>(dg.p, narrow<T, V>(og));
+      if (want_x) store_vec<T, V>(dx.p, narrow<T, V>(ox));
     }
     advance(dg.p, -dg.st);
     advance(dx.p, -dx.st);
   }
+  carry = pass * carry;
 }
 
-// Backward: tiles and chunks from the last to the first, the carried value the gradient of the state
+// Backward: chunks from the segment's last to its first, the carried value the gradient of the state
 // before the steps already done.
-template <typename T, int V, bool GATED, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT ? 32 * MAX_WARPS : 32 * WIDE_WARPS, SPLIT ? 1 : WIDE_GRAD_BLOCKS)
-    k_scan_grad(const __grid_constant__ Args p, int blocks) {
-  const int warp = threadIdx.x >> 5, warps = SPLIT ? blockDim.x >> 5 : 1;
-  const int rank = SPLIT ? (int)(blockIdx.x % blocks) : 0;
-  const int64_t group = SPLIT ? blockIdx.x / blocks : (int64_t)blockIdx.x * WIDE_WARPS + warp;
-  const Lane l = lane_of(p, (group * 32 + (threadIdx.x & 31)) * V);
-  const int T_ = (int)p.steps, chunks = (T_ + CHUNK - 1) / CHUNK, tile = SPLIT ? warps * blocks : 1;
-  float carry[V];
-  load_state<V>(carry, p.dhn, l);
-  if (SPLIT && blocks > 1) cg::this_cluster().sync();
-  int half = 0;
-  for (int done = 0; done < chunks; done += tile, half ^= 1) {
-    const int q = chunks - 1 - (done + (SPLIT ? rank * warps + warp : 0));      // below 0: nothing left
-    const int t0 = q * CHUNK, left = q < 0 ? 0 : T_ - t0;
-    const int n = l.live && q >= 0 ? (l.len - t0 < CHUNK ? l.len - t0 : CHUNK) : 0;
-    const bool all = __all_sync(~0u, n == CHUNK);
-    Vec<T, V> g[CHUNK], x[CHUNK], dh[CHUNK];
-    load_chunk<T, V>(g, Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
-    if (p.dh) {
-      load_chunk<T, V>(dh, Line<T>(p.dh, p.dh_t, p.dh_b, l, t0), n, all);
-    } else {
-#pragma unroll
-      for (int i = 0; i < CHUNK; i++)
-#pragma unroll
-        for (int k = 0; k < V; k++) dh[i].e[k] = from_f32<T>(0.0f);
-    }
-    load_chunk<T, V>(x, Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
-    const unsigned cut = resets_of(p, l, t0, n);
+template <typename T, int V, bool GATED>
+__global__ void __launch_bounds__(32 * WARPS, GRAD_BLOCKS)
+    k_scan_grad(const __grid_constant__ Args p, const __grid_constant__ Shape sh) {
+  constexpr bool STAGED = V * sizeof(T) == 4;
+  typedef Inputs<T, V, STAGED> In;
+  typedef typename Lanes<V>::type P;
+  __shared__ __align__(16) typename In::Buffer buffer;
+  int segment;
+  Lane l;
+  if (!task_of(p, sh, V, sh.maps, segment, l)) return;
+  const int steps = (int)p.steps, begin = segment * sh.length;
+  const int end = steps - begin < sh.length ? steps : begin + sh.length;
+  const int64_t channels = p.batch * p.dim;
+  P carry = load_state<V>(end < steps ? sh.starts + segment * channels : p.dhn, l);
+  In in(buffer, p, l);
+  int stage = 0;
+  const int first = begin + (end - begin - 1) / CHUNK * CHUNK;
+  const auto saved_at = [&](int t0) {
+    return load_state<V>(t0 >= begin && steps_of(l, t0) > 0 ? p.saved + (int64_t)(t0 / CHUNK) * channels : nullptr, l);
+  };
+  if constexpr (STAGED) in.fetch(p, l, 0, first, steps_of(l, first));
+  P h = saved_at(first), h_next = h;
+  bool ahead = reset_ahead(p, l, first);
+  for (int t0 = first; t0 >= begin; t0 -= CHUNK, h = h_next) {
+    const int n = steps_of(l, t0), left = steps - t0, next = t0 - CHUNK;
+    const unsigned cut = resets_of(p, l, t0, n, ahead);
+    if constexpr (STAGED) in.fetch(p, l, stage ^ 1, next, next >= begin ? steps_of(l, next) : 0);
+    h_next = saved_at(next);
+    if (next >= begin) ahead = reset_ahead(p, l, next);
+    if constexpr (STAGED) in.wait();
+    else in.load(p, l, t0, n);
     const bool plain = __all_sync(~0u, n == CHUNK && cut == 0);
-    float h[V], c_in[V];
-    load_state<V>(h, n > 0 ? p.saved + (int64_t)q * p.batch * p.dim : nullptr, l);
-    float s[GATED ? CHUNK : 1][V];
-    pack_gates<T, V, GATED>(g, s);
-    if (SPLIT) {
-      __shared__ Shared<V> sh;
-      float A[V], B[V];
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        A[k] = 1.0f;
-        B[k] = 0.0f;
-      }
-#pragma unroll
-      for (int i = CHUNK - 1; i >= 0; i--) {
-        float gf[V], df[V];
-        unpack<T, V>(dh[i], df);
-        if (!GATED) unpack<T, V>(g[i], gf);
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-          float a, c;
-          coefficients<GATED>(GATED ? s[i][k] : gf[k], a, c);
-          if (i < n) {
-            const bool r = cut >> i & 1;
-            A[k] = r ? __int_as_float(0x7fffffff) : A[k] * a;
-            B[k] = r ? 0.0f : a * (df[k] + B[k]);
-          }
-        }
-      }
-      join<V>(sh, half, warps, blocks, rank, A, B, carry, c_in);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; k++) c_in[k] = carry[k];
-    }
     const Line<T> dg(p.dgate, p.dgate_t, p.dgate_b, l, t0), dx(p.dx, p.dx_t, p.dx_b, l, t0);
     const bool want_g = p.dgate, want_x = p.dx;
-    if (plain) walk_back<T, V, GATED, true>(g, s, x, dh, 0, CHUNK, CHUNK, true, dg, want_g, dx, want_x, h, c_in);
-    else walk_back<T, V, GATED, false>(g, s, x, dh, cut, n, left, l.live, dg, want_g, dx, want_x, h, c_in);
-    if (!SPLIT) {
-#pragma unroll
-      for (int k = 0; k < V; k++) carry[k] = c_in[k];
-    }
+    if (plain) walk_back<T, V, GATED, true>(in, stage, 0, CHUNK, CHUNK, true, dg, want_g, dx, want_x, h, carry);
+    else walk_back<T, V, GATED, false>(in, stage, cut, n, left, l.live, dg, want_g, dx, want_x, h, carry);
+    stage ^= 1;
   }
-  if (!SPLIT || (rank == 0 && warp == 0)) store_state<V>(p.dh0, carry, l);
+  if (begin == 0) store_state<V>(p.dh0, carry, l);
 }
 
 // One step over [batch][dim], the fp32 state updated in place: elementwise, V values a thread.
@@ -531,9 +585,8 @@ __global__ void __launch_bounds__(256)
   Vec<T, V> o;
 #pragma unroll
   for (int k = 0; k < V; k++) {
-    float a, c;
-    coefficients<GATED>(packed_gate<GATED>(to_f32(g.e[k])), a, c);
-    const float b = GATED ? c * to_f32(xv.e[k]) : to_f32(xv.e[k]);
+    float a, b, c;
+    step_of<GATED>(to_f32(g.e[k]), to_f32(xv.e[k]), a, b, c);
     h[k] = cut ? b : fmaf(a, h[k], b);
     o.e[k] = from_f32<T>(h[k]);
   }
@@ -547,52 +600,47 @@ __global__ void __launch_bounds__(256)
   store_vec<T, V>(out + row * out_b + d, o);
 }
 
-// Warps that keep an SM's loads going; fewer channel groups than this many on every SM and the work is
-// split along time as well.
-constexpr int WARPS_PER_SM = 16;
-
-struct Shape {
-  bool split;
-  int warps, blocks;      // on consecutive chunks: of a block, of a cluster
-  int64_t grid;
-};
-
+// Segments: a multiple of CHUNK steps, few enough that the fold's and the walk's warps fill the GPU.
 inline Shape shape_for(int64_t channels, int64_t steps, int v) {
-  const int64_t groups = (channels + 32 * v - 1) / (32 * v), want = (int64_t)sm_count() * WARPS_PER_SM;
-  const int64_t chunks = (steps + CHUNK - 1) / CHUNK;
-  Shape s = {false, 1, 1, (groups + WIDE_WARPS - 1) / WIDE_WARPS};
-  if (chunks == 1 || groups * 2 > want) return s;
-  s.split = true;
-  while (s.warps < MAX_WARPS && s.warps < chunks && groups * s.warps < want) s.warps *= 2;
-  while (s.blocks < MAX_CLUSTER && s.warps * s.blocks < chunks && groups * s.warps * s.blocks < want) s.blocks *= 2;
-  if (s.blocks > s.warps) s.blocks = s.warps;
-  s.grid = groups * s.blocks;
+  Shape s = {(channels + 32 * v - 1) / (32 * v), 1, (int)((steps + CHUNK - 1) / CHUNK * CHUNK), nullptr, nullptr};
+  const int64_t want = (int64_t)sm_count() * WARPS_PER_SM, chunks = (steps + CHUNK - 1) / CHUNK;
+  if (s.groups * 2 > want || chunks < 2) return s;
+  const int64_t cuts = (want + s.groups - 1) / s.groups;                 // at least two
+  int64_t each = (chunks + cuts - 1) / cuts;                             // chunks of a segment
+  if (each > MAX_SEGMENT / CHUNK) each = MAX_SEGMENT / CHUNK;
+  s.length = (int)each * CHUNK;
+  s.segments = (int)((chunks + each - 1) / each);
   return s;
 }
 
-template <typename K>
-int launch(K kernel, const Args& p, const Shape& s, cudaStream_t st) {
-  if (s.grid > 0x7fffffff) return F16_ERR_TOO_LARGE;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)s.grid);
-  cfg.blockDim = dim3(32 * (s.split ? s.warps : WIDE_WARPS));
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  if (s.blocks > 1) {
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)s.blocks, 1, 1};
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-  }
-  (void)cudaLaunchKernelEx(&cfg, kernel, p, s.blocks);
-  return launch_status();
-}
+inline int64_t scratch_for(const Shape& s, int64_t channels) { return s.segments > 1 ? 3 * s.segments * channels : 0; }
 
 template <typename T, int V, bool GATED>
 int run(const Args& p, bool grad, cudaStream_t st) {
-  const Shape s = shape_for(p.batch * p.dim, p.steps, V);
-  if (grad) return s.split ? launch(k_scan_grad<T, V, GATED, true>, p, s, st) : launch(k_scan_grad<T, V, GATED, false>, p, s, st);
-  return s.split ? launch(k_scan<T, V, GATED, true>, p, s, st) : launch(k_scan<T, V, GATED, false>, p, s, st);
+  const int64_t channels = p.batch * p.dim;
+  Shape s = shape_for(channels, p.steps, V);
+  if (s.segments > 1 && p.scratch && p.scratch_floats >= scratch_for(s, channels)) {
+    s.maps = reinterpret_cast<float2*>(p.scratch);
+    s.starts = p.scratch + 2 * s.segments * channels;
+  } else {
+    s.segments = 1;
+    s.length = (int)((p.steps + CHUNK - 1) / CHUNK * CHUNK);
+  }
+  const int64_t grid = (s.groups * s.segments + WARPS - 1) / WARPS, starts = (channels + 31) / 32;
+  if (grid > 0x7fffffff) return F16_ERR_TOO_LARGE;
+  const unsigned blocks = (unsigned)grid, threads = 32 * WARPS;
+  if (s.maps) {
+    if (grad) {
+      k_scan_fold<T, V, GATED, true><<<blocks, threads, 0, st>>>(p, s);
+      k_scan_starts<true><<<(unsigned)starts, 32 * START_WARPS, 0, st>>>(s, channels, p.dhn);
+    } else {
+      k_scan_fold<T, V, GATED, false><<<blocks, threads, 0, st>>>(p, s);
+      k_scan_starts<false><<<(unsigned)starts, 32 * START_WARPS, 0, st>>>(s, channels, p.h0);
+    }
+  }
+  if (grad) k_scan_grad<T, V, GATED><<<blocks, threads, 0, st>>>(p, s);
+  else k_scan<T, V, GATED><<<blocks, threads, 0, st>>>(p, s);
+  return launch_status();
 }
 
 template <typename T, int V>
@@ -619,10 +667,11 @@ inline int check(const Args* p, bool grad) {
     return F16_ERR_ARG;
   if (p->dtype != F16_DTYPE_BF16 && p->dtype != F16_DTYPE_FP16 && p->dtype != F16_DTYPE_FP32) return F16_ERR_ARG;
   if (grad ? !p->saved || (!p->dh && !p->dhn) : !p->h) return F16_ERR_ARG;
-  if (p->steps > 0x7fffffff - 32 * CHUNK * MAX_WARPS * MAX_CLUSTER) return F16_ERR_TOO_LARGE;
+  if (p->steps > 0x7fffffff - 2 * CHUNK || p->batch > INT64_MAX / 16 / p->dim) return F16_ERR_TOO_LARGE;
   const int size = p->dtype == F16_DTYPE_FP32 ? 4 : 2;
   if (!aligned(p->gate, size) || !aligned(p->x, size) || !aligned(p->h, size) || !aligned(p->dh, size) ||
-      !aligned(p->dgate, size) || !aligned(p->dx, size) || (p->reset_bytes == 4 && !aligned(p->reset, 4)))
+      !aligned(p->dgate, size) || !aligned(p->dx, size) || (p->reset && p->reset_bytes == 4 && !aligned(p->reset, 4)) ||
+      !aligned(p->scratch, 8))
     return F16_ERR_ALIGN;
   return F16_OK;
 }
@@ -661,6 +710,13 @@ using namespace f16;
 extern "C" int64_t f16_scan_saved_floats(int64_t steps, int64_t batch, int64_t dim) {
   if (steps <= 0 || batch <= 0 || dim <= 0) return 0;
   return (steps + scan::CHUNK - 1) / scan::CHUNK * batch * dim;
+}
+
+extern "C" int64_t f16_scan_scratch_floats(int64_t steps, int64_t batch, int64_t dim) {
+  if (steps <= 0 || batch <= 0 || dim <= 0 || batch > INT64_MAX / 16 / dim) return 0;
+  const int64_t one = scan::scratch_for(scan::shape_for(batch * dim, steps, 1), batch * dim),
+                two = scan::scratch_for(scan::shape_for(batch * dim, steps, 2), batch * dim);
+  return one > two ? one : two;
 }
 
 extern "C" int f16_scan_fwd(const f16_scan_args* args, f16_stream_t stream) { return scan::go(args, false, stream); }

@@ -46,11 +46,18 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
-def _args(gate, x, h0, reset, lengths, gated, h, hn, saved, dh=None, dhn=None, dgate=None, dx=None, dh0=None):
+def _scratch(lib, x):
+    """(buffer, values in it) for the segments of a scan with few channels, or (None, 0)."""
+    n = lib.f16_scan_scratch_floats(*x.shape)
+    return (torch.empty(n, dtype=torch.float32, device=x.device) if n else None), n
+
+
+def _args(gate, x, h0, reset, lengths, gated, h, hn, saved, scratch, dh=None, dhn=None, dgate=None, dx=None, dh0=None):
     return _lib.ScanArgs(_lib.DTYPES[x.dtype], gated, *x.shape, *_place(gate), *_place(x), _at(h0), _at(reset),
                          reset.element_size() if reset is not None else 0,
                          *(reset.stride() if reset is not None else (0, 0)), _at(lengths), *_place(h), _at(hn), _at(saved),
-                         *_place(dh), _at(dhn), *_place(dgate), *_place(dx), _at(dh0))
+                         *_place(dh), _at(dhn), *_place(dgate), *_place(dx), _at(dh0),
+                         _at(scratch[0]), scratch[1])
 
 
 def _forward(gate, x, h0, reset, lengths, gated, keep):
@@ -65,8 +72,9 @@ def _forward(gate, x, h0, reset, lengths, gated, keep):
         lib = _lib.load()
         if keep:
             saved = torch.empty(lib.f16_scan_saved_floats(steps, batch, dim), dtype=torch.float32, device=x.device)
-        a = _args(gate, x, h0, reset, lengths, gated, h, hn, saved)
         with _lib.on_device(x):
+            scratch = _scratch(lib, x)
+            a = _args(gate, x, h0, reset, lengths, gated, h, hn, saved, scratch)
             _lib.check(lib.f16_scan_fwd(C.byref(a), _lib.raw_stream(x)), "f16_scan_fwd")
     return h, hn, saved
 
@@ -97,9 +105,11 @@ class _Scan(torch.autograd.Function):
             return dgate, dx, dh0, None, None, None
         dh = _strided(dh) if dh is not None else None
         dhn = dhn.contiguous() if dhn is not None else None
-        a = _args(gate, x, h0, reset, lengths, ctx.gated, None, None, saved, dh, dhn, dgate, dx, dh0)
+        lib = _lib.load()
         with _lib.on_device(x):
-            _lib.check(_lib.load().f16_scan_bwd(C.byref(a), _lib.raw_stream(x)), "f16_scan_bwd")
+            scratch = _scratch(lib, x)
+            a = _args(gate, x, h0, reset, lengths, ctx.gated, None, None, saved, scratch, dh, dhn, dgate, dx, dh0)
+            _lib.check(lib.f16_scan_bwd(C.byref(a), _lib.raw_stream(x)), "f16_scan_bwd")
         return dgate, dx, dh0, None, None, None
 
 
@@ -133,7 +143,7 @@ def gated_scan(gate, x, h0=None, reset=None, lengths=None):
 
 def linear_scan(a, x, h0=None, reset=None, lengths=None):
     """(h, hn) of h_t = a_t h_{t-1} + x_t; arguments as in ``gated_scan``.  Meant for coefficients of
-    size up to 1; the product of 256 successive ones has to stay in fp32's range."""
+    size up to 1; the product of 512 successive ones has to stay in fp32's range."""
     return _scan(a, x, h0, reset, lengths, False, "linear_scan")
 
 

@@ -550,9 +550,11 @@ int64_t f16_layer_norm_scratch_floats(int64_t rows, int cols);
  * The forward pass writes `saved` (f16_scan_saved_floats values, or NULL where no gradient follows): the
  * state before every F16_SCAN_CHUNK steps.  The backward pass reads it with gate, x and the gradients
  * dh and dhn (one of them may be NULL: zero) and writes dgate, dx and dh0, each NULL where not
- * wanted.  Coefficients above 1 in size: the product of any F16_SCAN_CHUNK x 16 successive ones has
- * to stay in fp32's range. */
+ * wanted.  scratch: f16_scan_scratch_floats values, 8-byte aligned (none of them are kept); with less or
+ * NULL, time is not cut into segments, which is slow for few channels and many steps.  Coefficients
+ * above 1 in size: the product of any F16_SCAN_SEGMENT successive ones has to stay in fp32's range. */
 #define F16_SCAN_CHUNK 16
+#define F16_SCAN_SEGMENT 512
 typedef struct {
   int dtype;                   /* of gate, x, h and their gradients */
   int gated;
@@ -578,7 +580,10 @@ typedef struct {
   void* dx;
   int64_t dx_t, dx_b;
   float* dh0;
+  float* scratch;
+  int64_t scratch_floats;
 } f16_scan_args;
+int64_t f16_scan_scratch_floats(int64_t steps, int64_t batch, int64_t dim);
 int64_t f16_scan_saved_floats(int64_t steps, int64_t batch, int64_t dim);
 int f16_scan_fwd(const f16_scan_args* args, f16_stream_t stream);
 int f16_scan_bwd(const f16_scan_args* args, f16_stream_t stream);

@@ -130,7 +130,8 @@ def test_many_channels(cuda, batch, dim, dtype, gated):
 
 @pytest.mark.parametrize("steps,batch,dim", [(100, 4, 64), (30, 3000, 64)])
 def test_reset_types_and_strides(cuda, steps, batch, dim):
-    """bool, uint8 and fp32 flags give the same bits, as do strided, sliced and batch-first inputs."""
+    """bool, uint8 and fp32 flags give the same bits, as do strides along time and batch; an input off the
+    alignment of pairs takes other kernels (and cuts time elsewhere), within the tolerance."""
     rec = pkg_module("recurrence")
     d, dh, dhn = make(cuda, steps, batch, dim, torch.bfloat16, True, 5, resets=True)
     want = run(d, True, dh, dhn)
@@ -144,8 +145,10 @@ def test_reset_types_and_strides(cuda, steps, batch, dim):
     two = torch.zeros(2 * steps, batch, dim, device=cuda, dtype=torch.bfloat16)
     two[::2] = d["gate"]
     dhs = dh.transpose(0, 1).contiguous().transpose(0, 1)
-    got = run({**d, "reset": flipped, "x": odd, "gate": two[::2]}, True, dhs, dhn)
+    got = run({**d, "reset": flipped, "gate": two[::2]}, True, dhs, dhn)
     assert all(torch.equal(got[n], want[n]) for n in want)
+    ref, tol = reference(d, True, dh, dhn)
+    check(run({**d, "x": odd}, True, dh, dhn), ref, tol)
     h, _ = rec.gated_scan(d["gate"].transpose(0, 1).contiguous().transpose(0, 1),
                           d["x"].transpose(0, 1).contiguous().transpose(0, 1), d["h0"], reset=d["reset"])
     assert torch.equal(h, want["h"]) and h.stride(0) < h.stride(1)      # batch-first in, batch-first out
