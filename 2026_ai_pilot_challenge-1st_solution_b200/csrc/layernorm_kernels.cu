@@ -18,9 +18,12 @@ namespace f16 {
 namespace ln {
 
 constexpr int BLOCK = 256;          // threads of a block whose rows take a warp or less
-constexpr int MAX_LANES = 512;     // threads of a row: 128 registers each
-constexpr int E = 16;               // most values of a row in one thread
+constexpr int MAX_LANES = 512;      // threads of a row: 128 registers each
+// Values of a row in one thread: 16, or 8 where loads are narrower than 16 bytes and the row's threads suffice.
+constexpr int MOST = 16;
 constexpr int WIDE = 1024;          // threads of a block on a row too wide for registers
+
+constexpr int threads_of(int lanes) { return lanes > 32 ? lanes : BLOCK; }
 
 struct Weights {
   const void* w;
@@ -39,211 +42,370 @@ __device__ __forceinline__ void store_from_f32(void* p, int dtype, int64_t i, fl
   else reinterpret_cast<__half*>(p)[i] = from_f32<__half>(v);
 }
 
-// Sum over the `lanes` threads of a row (xor shuffles: every thread gets the same bits).  Rows wider
-// than a warp take the whole block and `red`; consecutive calls alternate its halves, so one barrier
-// a call is enough.
-__device__ __forceinline__ float row_sum(float v, int lanes, float (*red)[32], int& half) {
-  const int w = lanes < 32 ? lanes : 32;
-  for (int o = w >> 1; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  if (lanes > 32) {
-    float* r = red[half];
-    half ^= 1;
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
-    __syncthreads();
-    const int n = lanes >> 5, l = threadIdx.x & 31;
-    v = l < n ? r[l] : 0.0f;
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+// Sums over the threads of a row (xor shuffles: every thread gets the same bits).  LANES: 1 to 16 at run
+// time (0), 32, or a block of 64 to 512, whose warps meet in `red`; consecutive calls alternate its halves,
+// so one barrier a call is enough.
+template <int LANES, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*red)[N][32], int& half) {
+  if constexpr (LANES == 0) {
+    for (int o = lanes >> 1; o; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(~0u, v[k], o);
+  } else {
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(~0u, v[k], o);
   }
-  return v;
+  if constexpr (LANES > 32) {
+    constexpr int W = LANES / 32;
+    float (*r)[32] = red[half];
+    half ^= 1;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < N; k++) r[k][threadIdx.x >> 5] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; k++) v[k] = r[k][threadIdx.x & (W - 1)];
+#pragma unroll
+    for (int o = W / 2; o; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(~0u, v[k], o);
+  }
 }
 
-template <typename T, int V, int NV>
-__device__ __forceinline__ void load_row(Vec<T, V> (&v)[NV], const T* row, bool live, int lane, int lanes, int cols) {
+// A thread's part of a row: NV loads of V values, `apart` values from one load to the next; bit j of `there`:
+// load j lies in the row.  The others read as zero.
+template <typename T, int V, int E>
+struct Part {
+  static constexpr int NV = E / V;
+  Vec<T, V> v[NV];
+  __device__ __forceinline__ void load(const T* p, int apart, unsigned there, bool full) {
+    if (full) {
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
-    const int c = (j * lanes + lane) * V;
-    if (live && c < cols) {
-      v[j] = load_vec_nc<T, V>(row + c);
+      for (int j = 0; j < NV; j++) v[j] = load_vec_nc<T, V>(p + j * apart);
     } else {
 #pragma unroll
-      for (int k = 0; k < V; k++) v[j].e[k] = from_f32<T>(0.0f);
+      for (int j = 0; j < NV; j++) {
+        if (there >> j & 1) {
+          v[j] = load_vec_nc<T, V>(p + j * apart);
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; k++) v[j].e[k] = from_f32<T>(0.0f);
+        }
+      }
     }
   }
+  // The pair i of the thread's E values, and the way back.
+  __device__ __forceinline__ Two pair(int i) const {
+    if constexpr (V == 1) return two(to_f32(v[2 * i].e[0]), to_f32(v[2 * i + 1].e[0]));
+    else return pair_of<T, V>(v[2 * i / V], i % (V / 2));
+  }
+  __device__ __forceinline__ void set(int i, Two t) {
+    if constexpr (V == 1) {
+      const float2 f = split(t);
+      v[2 * i].e[0] = from_f32<T>(f.x);
+      v[2 * i + 1].e[0] = from_f32<T>(f.y);
+    } else {
+      set_pair<T, V>(v[2 * i / V], i % (V / 2), t);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int apart, unsigned there, bool full) const {
+    if (full) {
+#pragma unroll
+      for (int j = 0; j < NV; j++) store_vec<T, V>(p + j * apart, v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (there >> j & 1) store_vec<T, V>(p + j * apart, v[j]);
+    }
+  }
+};
+
+// The thread's parts of its next rows, N tensors' of each: on their way into shared memory two rows ahead
+// (one row a block in flight leaves HBM idle half of the time), or, where a load is narrower than the 4 bytes
+// that can be copied so, one row ahead in registers.  A thread reads what it copied itself, so no barrier.
+constexpr int SLOTS = 3;
+template <typename T, int V, int E, int N>
+struct Ring {
+  static constexpr bool STAGED = V * sizeof(T) >= 4;
+  static constexpr int NV = E / V, BYTES = V * (int)sizeof(T);
+  typedef Vec<T, V> Unit;
+  Unit* slots;              // [SLOTS][N][NV][threads], this thread's
+  int threads, filled, taken;
+  Part<T, V, E> next[STAGED ? 1 : N];
+  static constexpr size_t bytes(int threads) { return STAGED ? (size_t)SLOTS * N * E * sizeof(T) * threads : 0; }
+  __device__ __forceinline__ Ring(unsigned char* smem, int threads, unsigned there) : threads(threads), filled(0), taken(0) {
+    slots = reinterpret_cast<Unit*>(smem) + threadIdx.x;
+    if constexpr (STAGED) {
+      if (there != (1u << NV) - 1) {      // what lies past the row's end is never copied: zero
+        Unit zero;
+#pragma unroll
+        for (int k = 0; k < V; k++) zero.e[k] = from_f32<T>(0.0f);
+#pragma unroll
+        for (int i = 0; i < SLOTS * N * NV; i++) slots[i * threads] = zero;
+      }
+    }
+  }
+  // Row `live` of every tensor into the next slot.
+  __device__ __forceinline__ void put(const T* const (&from)[N], int apart, unsigned there, bool full) {
+    if constexpr (STAGED) {
+      const unsigned to = (unsigned)__cvta_generic_to_shared(slots + filled * N * NV * threads);
+#pragma unroll
+      for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+          if (full || there >> j & 1) {
+            const unsigned at = to + (n * NV + j) * threads * BYTES;
+            if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from[n] + j * apart) : "memory");
+            else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from[n] + j * apart), "n"(BYTES) : "memory");
+          }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      filled = filled + 1 == SLOTS ? 0 : filled + 1;
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; n++) next[n].load(from[n], apart, there, full);
+    }
+  }
+  __device__ __forceinline__ void take(Part<T, V, E> (&row)[N]) {
+    if constexpr (STAGED) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 2) : "memory");
+#pragma unroll
+      for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int j = 0; j < NV; j++) row[n].v[j] = slots[((taken * N + n) * NV + j) * threads];
+      taken = taken + 1 == SLOTS ? 0 : taken + 1;
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; n++) row[n] = next[n];
+    }
+  }
+};
+
+// Where a thread works: its row's place in the block, its first column, what it has of a row.
+template <int V, int E, int LANES>
+struct Place {
+  int lanes, lane, group, per, apart;
+  unsigned there;
+  bool full;                    // every thread of the row has all its values
+  __device__ __forceinline__ Place(int cols, int run_lanes) {
+    lanes = LANES ? LANES : run_lanes;
+    lane = threadIdx.x & (lanes - 1);
+    group = LANES > 32 ? 0 : threadIdx.x / lanes;
+    per = LANES > 32 ? 1 : BLOCK / lanes;
+    apart = lanes * V;
+    there = 0;
+#pragma unroll
+    for (int j = 0; j < E / V; j++) there |= (unsigned)((j * lanes + lane) * V < cols) << j;
+    full = cols == E * lanes;
+  }
+  // The column of value e of the thread.
+  __device__ __forceinline__ int column(int e) const { return (e / V * lanes + lane) * V + e % V; }
+};
+
+__device__ __forceinline__ float sum_of(const Two (&s)[2]) {
+  const float2 f = split(s[0] + s[1]);
+  return f.x + f.y;
 }
 
-template <typename T, int V, int NV>
-__global__ void __launch_bounds__(MAX_LANES)
+template <typename T, int V, int E, int LANES>
+__global__ void __launch_bounds__(threads_of(LANES), 768 / threads_of(LANES))
     k_ln_fwd(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps, T* __restrict__ y,
              int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd, int lanes) {
-  __shared__ float red[2][32];
+  __shared__ float red[2][1][32];
   int half = 0;
-  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, per = blockDim.x / lanes;
-  const int64_t step = (int64_t)gridDim.x * per;
-  float w[NV][V], b[NV][V];
+  const Place<V, E, LANES> at(cols, lanes);
+  const int64_t step = (int64_t)gridDim.x * at.per;
+  Two w[E / 2], b[E / 2];
 #pragma unroll
-  for (int j = 0; j < NV; j++)
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-      const int c = (j * lanes + lane) * V + k;
-      w[j][k] = wb.w && c < cols ? load_as_f32(wb.w, wb.dtype, c) : 1.0f;
-      b[j][k] = wb.b && c < cols ? load_as_f32(wb.b, wb.dtype, c) : 0.0f;
-    }
-  Vec<T, V> next[NV];
-  int64_t r0 = (int64_t)blockIdx.x * per;
-  load_row<T, V, NV>(next, x + (r0 + group) * ldx, r0 + group < rows, lane, lanes, cols);
+  for (int i = 0; i < E / 2; i++) {
+    const int c0 = at.column(2 * i), c1 = at.column(2 * i + 1);
+    w[i] = two(wb.w && c0 < cols ? load_as_f32(wb.w, wb.dtype, c0) : 1.0f, wb.w && c1 < cols ? load_as_f32(wb.w, wb.dtype, c1) : 1.0f);
+    b[i] = two(wb.b && c0 < cols ? load_as_f32(wb.b, wb.dtype, c0) : 0.0f, wb.b && c1 < cols ? load_as_f32(wb.b, wb.dtype, c1) : 0.0f);
+  }
+  int64_t row = (int64_t)blockIdx.x * at.per + at.group;
+  T* to = y + row * ldy + at.lane * V;
   const float inv = 1.0f / (float)cols;
-  for (; r0 < rows; r0 += step) {
-    const int64_t row = r0 + group;
-    const bool live = row < rows;
-    float v[NV][V], s = 0.0f;
+  typedef Ring<T, V, E, 1> Rows;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Rows ring(smem, threads_of(LANES), at.there);
+  const T* from[1] = {x + row * ldx + at.lane * V};
+  int64_t ahead = row;
+  const auto put = [&] {
+    const bool live = ahead < rows;
+    ring.put(from, at.apart, live ? at.there : 0u, at.full && live);
+    from[0] += step * ldx;
+    ahead += step;
+  };
+  put();
+  if (Rows::STAGED) put();
+  // every thread of a warp (or block) makes the same number of rounds: the sums are theirs together
+  for (int64_t first = (int64_t)blockIdx.x * at.per; first < rows; first += step, row += step, to += step * ldy) {
+    Part<T, V, E> here[1];
+    ring.take(here);
+    put();
+    Two v[E / 2], s[2] = {two(0.0f), two(0.0f)};
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        v[j][k] = to_f32(next[j].e[k]);
-        s += v[j][k];
-      }
-    load_row<T, V, NV>(next, x + (row + step) * ldx, row + step < rows, lane, lanes, cols);
-    const float mu = row_sum(s, lanes, red, half) * inv;
-    float q = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; j++)
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        v[j][k] -= mu;
-        if ((j * lanes + lane) * V < cols) q = fmaf(v[j][k], v[j][k], q);
-      }
-    const float r = 1.0f / sqrtf(row_sum(q, lanes, red, half) * inv + eps);
-    if (!live) continue;
-    if (lane == 0 && mean) {
-      mean[row] = mu;
-      rstd[row] = r;
+    for (int i = 0; i < E / 2; i++) {
+      v[i] = here[0].pair(i);
+      s[i & 1] = s[i & 1] + v[i];
     }
+    float total[1] = {sum_of(s)};
+    row_sums<LANES, 1>(total, at.lanes, red, half);
+    const float mu = total[0] * inv;
+    const Two minus = two(-mu);
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-      const int c = (j * lanes + lane) * V;
-      Vec<T, V> o;
+    for (int i = 0; i < E / 2; i++) v[i] = v[i] + minus;
+    if (!at.full) {              // what lies past the row's end is zero, not the mean's negative
 #pragma unroll
-      for (int k = 0; k < V; k++) o.e[k] = from_f32<T>(fmaf(v[j][k] * r, w[j][k], b[j][k]));
-      if (c < cols) store_vec<T, V>(y + row * ldy + c, o);
+      for (int i = 0; i < E / 2; i++) {
+        const float2 f = split(v[i]);
+        v[i] = two(at.there >> (2 * i / V) & 1 ? f.x : 0.0f, at.there >> ((2 * i + 1) / V) & 1 ? f.y : 0.0f);
+      }
+    }
+    s[0] = s[1] = two(0.0f);
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) s[i & 1] = fma2(v[i], v[i], s[i & 1]);
+    total[0] = sum_of(s);
+    row_sums<LANES, 1>(total, at.lanes, red, half);
+    const float r = rsqrtf(total[0] * inv + eps);
+    if (row < rows) {
+      if (at.lane == 0 && mean) {
+        mean[row] = mu;
+        rstd[row] = r;
+      }
+      Part<T, V, E> out;
+      const Two scale = two(r);
+#pragma unroll
+      for (int i = 0; i < E / 2; i++) out.set(i, fma2(v[i] * scale, w[i], b[i]));
+      out.store(to, at.apart, at.there, at.full);
     }
   }
 }
 
 // Backward of the rows of one block, and its columns' sums part[block][0][cols] (dw) and
 // part[block][1][cols] (db).  dx or part may be null.
-template <typename T, int V, int NV>
-__global__ void __launch_bounds__(MAX_LANES)
+template <typename T, int V, int E, int LANES>
+__global__ void __launch_bounds__(threads_of(LANES), 512 / threads_of(LANES))
     k_ln_bwd(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ x, int64_t ldx, int64_t rows, int cols,
              Weights wb, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
              int64_t ldd, float* __restrict__ part, int lanes) {
-  __shared__ float red[2][32];
-  extern __shared__ float col_sum[];            // 2 cols floats where several rows share the block
+  __shared__ float red[2][2][32];
+  extern __shared__ __align__(16) unsigned char smem[];
   int half = 0;
-  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, per = blockDim.x / lanes;
-  const int64_t step = (int64_t)gridDim.x * per;
-  float w[NV][V], aw[NV][V], ab[NV][V];
+  const Place<V, E, LANES> at(cols, lanes);
+  const int64_t step = (int64_t)gridDim.x * at.per;
+  Two w[E / 2], aw[E / 2], ab[E / 2];
 #pragma unroll
-  for (int j = 0; j < NV; j++)
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-      const int c = (j * lanes + lane) * V + k;
-      w[j][k] = wb.w && c < cols ? load_as_f32(wb.w, wb.dtype, c) : 1.0f;
-      aw[j][k] = ab[j][k] = 0.0f;
-    }
-  Vec<T, V> nx[NV], ng[NV];
-  float nmu = 0.0f, nr = 0.0f;
-  int64_t r0 = (int64_t)blockIdx.x * per;
-  const auto fetch = [&](int64_t row) {
-    const bool live = row < rows;
-    load_row<T, V, NV>(nx, x + row * ldx, live, lane, lanes, cols);
-    load_row<T, V, NV>(ng, dy + row * ldg, live, lane, lanes, cols);
-    nmu = live ? mean[row] : 0.0f;
-    nr = live ? rstd[row] : 0.0f;
-  };
-  fetch(r0 + group);
+  for (int i = 0; i < E / 2; i++) {
+    const int c0 = at.column(2 * i), c1 = at.column(2 * i + 1);
+    w[i] = two(wb.w && c0 < cols ? load_as_f32(wb.w, wb.dtype, c0) : 1.0f, wb.w && c1 < cols ? load_as_f32(wb.w, wb.dtype, c1) : 1.0f);
+    aw[i] = ab[i] = two(0.0f);
+  }
+  int64_t row = (int64_t)blockIdx.x * at.per + at.group;
+  T* to = dx ? dx + row * ldd + at.lane * V : nullptr;
   const float inv = 1.0f / (float)cols;
-  for (; r0 < rows; r0 += step) {
-    const int64_t row = r0 + group;
-    const bool live = row < rows;
-    const float mu = nmu, r = nr;
-    Vec<T, V> cx[NV], cg[NV];
+  typedef Ring<T, V, E, 2> Rows;
+  Rows ring(smem, threads_of(LANES), at.there);
+  const T* from[2] = {x + row * ldx + at.lane * V, dy + row * ldg + at.lane * V};
+  int64_t ahead = row;
+  const auto put = [&] {
+    const bool live = ahead < rows;
+    ring.put(from, at.apart, live ? at.there : 0u, at.full && live);
+    from[0] += step * ldx;
+    from[1] += step * ldg;
+    ahead += step;
+  };
+  put();
+  if (Rows::STAGED) put();
+  float nmu = row < rows ? mean[row] : 0.0f, nr = row < rows ? rstd[row] : 0.0f;
+  for (int64_t first = (int64_t)blockIdx.x * at.per; first < rows; first += step, row += step, to += step * ldd) {
+    Part<T, V, E> here[2];
+    ring.take(here);
+    put();
+    const Part<T, V, E>&cx = here[0], &cg = here[1];
+    const Two minus = two(-nmu), scale = two(nr);
+    const float r = nr;
+    nmu = row + step < rows ? mean[row + step] : 0.0f;
+    nr = row + step < rows ? rstd[row + step] : 0.0f;
+    Two s1 = two(0.0f), s2 = two(0.0f);
+    if (row < rows) {
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-      cx[j] = nx[j];
-      cg[j] = ng[j];
-    }
-    fetch(row + step);
-    float s1 = 0.0f, s2 = 0.0f;
-    if (live) {
-#pragma unroll
-      for (int j = 0; j < NV; j++)
-        if ((j * lanes + lane) * V < cols) {
-#pragma unroll
-          for (int k = 0; k < V; k++) {
-            const float xh = (to_f32(cx[j].e[k]) - mu) * r, d = to_f32(cg[j].e[k]), g = d * w[j][k];
-            s1 += g;
-            s2 = fmaf(g, xh, s2);
-            aw[j][k] = fmaf(d, xh, aw[j][k]);
-            ab[j][k] += d;
-          }
-        }
+      for (int i = 0; i < E / 2; i++) {
+        const Two d = cg.pair(i), xh = (cx.pair(i) + minus) * scale, g = d * w[i];
+        s1 = s1 + g;
+        s2 = fma2(g, xh, s2);
+        aw[i] = fma2(d, xh, aw[i]);
+        ab[i] = ab[i] + d;
+      }
     }
     if (!dx) continue;
-    const float m1 = row_sum(s1, lanes, red, half) * inv, m2 = row_sum(s2, lanes, red, half) * inv;
-    if (!live) continue;
+    const float2 f1 = split(s1), f2 = split(s2);
+    float total[2] = {f1.x + f1.y, f2.x + f2.y};
+    row_sums<LANES, 2>(total, at.lanes, red, half);
+    if (row < rows) {
+      // dx = r g - r m1 - xh r m2
+      const Two m1 = two(-total[0] * inv), m2 = two(-total[1] * inv), rr = two(r);
+      Part<T, V, E> out;
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-      const int c = (j * lanes + lane) * V;
-      Vec<T, V> o;
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        const float xh = (to_f32(cx[j].e[k]) - mu) * r, g = to_f32(cg[j].e[k]) * w[j][k];
-        o.e[k] = from_f32<T>(r * (g - m1 - xh * m2));
+      for (int i = 0; i < E / 2; i++) {
+        const Two xh = (cx.pair(i) + minus) * scale, g = cg.pair(i) * w[i];
+        out.set(i, fma2(xh, m2, g + m1) * rr);
       }
-      if (c < cols) store_vec<T, V>(dx + row * ldd + c, o);
+      out.store(to, at.apart, at.there, at.full);
     }
   }
   if (!part) return;
   float* out = part + (int64_t)blockIdx.x * 2 * cols;
-  if (per == 1) {
+  float sw[E], sb[E];
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        const int c = (j * lanes + lane) * V + k;
-        if (c < cols) {
-          out[c] = aw[j][k];
-          out[cols + c] = ab[j][k];
-        }
-      }
-    return;
+  for (int i = 0; i < E / 2; i++) {
+    split(aw[i], sw[2 * i], sw[2 * i + 1]);
+    split(ab[i], sb[2 * i], sb[2 * i + 1]);
   }
-  // rows of one warp first (shuffles), then the warps in turn
+  if constexpr (LANES > 32) {
 #pragma unroll
-  for (int j = 0; j < NV; j++)
-#pragma unroll
-    for (int k = 0; k < V; k++)
-      for (int o = 16; o >= lanes; o >>= 1) {
-        aw[j][k] += __shfl_xor_sync(~0u, aw[j][k], o);
-        ab[j][k] += __shfl_xor_sync(~0u, ab[j][k], o);
+    for (int e = 0; e < E; e++) {
+      const int c = at.column(e);
+      if (c < cols) {
+        out[c] = sw[e];
+        out[cols + c] = sb[e];
       }
-  for (int turn = 0; turn < (int)(blockDim.x >> 5); turn++) {
-    if ((int)(threadIdx.x >> 5) == turn && (int)(threadIdx.x & 31) < lanes) {
+    }
+  } else {
+    // rows of one warp first (shuffles), then the warps in turn, in the ring's memory
+    float* col_sum = reinterpret_cast<float*>(smem);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < NV; j++)
+    for (int e = 0; e < E; e++)
+      for (int o = 16; o >= at.lanes; o >>= 1) {
+        sw[e] += __shfl_xor_sync(~0u, sw[e], o);
+        sb[e] += __shfl_xor_sync(~0u, sb[e], o);
+      }
+    for (int turn = 0; turn < BLOCK / 32; turn++) {
+      if ((int)(threadIdx.x >> 5) == turn && (int)(threadIdx.x & 31) < at.lanes) {
 #pragma unroll
-        for (int k = 0; k < V; k++) {
-          const int c = (j * lanes + lane) * V + k;
+        for (int e = 0; e < E; e++) {
+          const int c = at.column(e);
           if (c < cols) {
-            col_sum[c] = turn ? col_sum[c] + aw[j][k] : aw[j][k];
-            col_sum[cols + c] = turn ? col_sum[cols + c] + ab[j][k] : ab[j][k];
+            col_sum[c] = turn ? col_sum[c] + sw[e] : sw[e];
+            col_sum[cols + c] = turn ? col_sum[cols + c] + sb[e] : sb[e];
           }
         }
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * cols; c += BLOCK) out[c] = col_sum[c];
   }
-  for (int c = threadIdx.x; c < 2 * cols; c += blockDim.x) out[c] = col_sum[c];
+}
+
+// The sum over a block of WIDE threads.
+__device__ __forceinline__ float wide_sum(float v, float (*red)[1][32], int& half) {
+  float t[1] = {v};
+  row_sums<WIDE, 1>(t, WIDE, red, half);
+  return t[0];
 }
 
 // Rows too wide for a block's registers: a block a row, read again for each of the three passes (the
@@ -252,19 +414,19 @@ template <typename T>
 __global__ void __launch_bounds__(WIDE)
     k_ln_fwd_wide(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps,
                   T* __restrict__ y, int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ float red[2][32];
+  __shared__ float red[2][1][32];
   int half = 0;
   const float inv = 1.0f / (float)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
     float s = 0.0f, q = 0.0f;
     for (int c = threadIdx.x; c < cols; c += WIDE) s += to_f32(xr[c]);
-    const float mu = row_sum(s, WIDE, red, half) * inv;
+    const float mu = wide_sum(s, red, half) * inv;
     for (int c = threadIdx.x; c < cols; c += WIDE) {
       const float d = to_f32(xr[c]) - mu;
       q = fmaf(d, d, q);
     }
-    const float r = 1.0f / sqrtf(row_sum(q, WIDE, red, half) * inv + eps);
+    const float r = rsqrtf(wide_sum(q, red, half) * inv + eps);
     if (threadIdx.x == 0 && mean) {
       mean[row] = mu;
       rstd[row] = r;
@@ -282,7 +444,7 @@ __global__ void __launch_bounds__(WIDE)
     k_ln_bwd_wide(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ x, int64_t ldx, int64_t rows, int cols,
                   Weights wb, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                   int64_t ldd, float* part) {
-  __shared__ float red[2][32];
+  __shared__ float red[2][1][32];
   int half = 0;
   const float inv = 1.0f / (float)cols;
   float* out = part ? part + (int64_t)blockIdx.x * 2 * cols : nullptr;
@@ -301,7 +463,7 @@ __global__ void __launch_bounds__(WIDE)
       }
     }
     if (!dx) continue;
-    const float m1 = row_sum(s1, WIDE, red, half) * inv, m2 = row_sum(s2, WIDE, red, half) * inv;
+    const float m1 = wide_sum(s1, red, half) * inv, m2 = wide_sum(s2, red, half) * inv;
     for (int c = threadIdx.x; c < cols; c += WIDE) {
       const float xh = (to_f32(x[row * ldx + c]) - mu) * r;
       const float g = to_f32(dy[row * ldg + c]) * (wb.w ? load_as_f32(wb.w, wb.dtype, c) : 1.0f);
@@ -332,33 +494,20 @@ __global__ void __launch_bounds__(1024) k_ln_wgrad(const float* __restrict__ par
   }
 }
 
-// How a row is spread: V values a load, NV loads and `lanes` threads a row; nv 0: the wide kernels.
+// How a row is spread: v values a load, e values a thread, `lanes` threads a row -- a power of two, the
+// fewest that hold it; 0: the wide kernels.
 struct Plan {
-  int v, nv, lanes, threads;
+  int v, e, lanes, threads;
 };
 
-inline int pow2_up(int n) {
-  int p = 1;
-  while (p < n) p <<= 1;
-  return p;
-}
-
 inline Plan plan_for(int cols, int v) {
-  Plan p;
-  p.v = v;
-  const int vecs = (cols + v - 1) / v;
-  // one value a load: 8 of them, so that a warp's request covers 32 neighbours before a row is
-  // spread over more of a thread's registers
-  const int most = v == 1 ? 8 : E / v;
-  p.lanes = pow2_up((vecs + most - 1) / most);
-  if (p.lanes > MAX_LANES) {
-    p.lanes = MAX_LANES;
-    p.nv = pow2_up((vecs + MAX_LANES - 1) / MAX_LANES);
-    if (p.nv * v > E) p.nv = 0;
-  } else {
-    p.nv = pow2_up((vecs + p.lanes - 1) / p.lanes);
-  }
-  p.threads = p.lanes > 32 ? p.lanes : BLOCK;
+  Plan p = {v, v > 2 || cols > MOST / 2 * MAX_LANES ? MOST : MOST / 2, 1, BLOCK};
+  while (p.lanes * p.e < cols) p.lanes <<= 1;
+  // one value a load: a warp's request should cover 32 neighbours before a thread takes many values
+  if (v == 1)
+    while (p.lanes < 32 && p.lanes < cols) p.lanes <<= 1;
+  if (p.lanes > MAX_LANES) p.lanes = 0;
+  p.threads = p.lanes > 32 ? p.lanes : p.lanes ? BLOCK : WIDE;
   return p;
 }
 
@@ -379,7 +528,36 @@ inline int64_t grid_rows(int64_t rows, const Plan& p, int warps_per_sm) {
   return need < most ? need : most;
 }
 
-constexpr int FWD_WARPS = 32, BWD_WARPS = 16;    // persistent warps per SM
+constexpr int FWD_WARPS = 24, BWD_WARPS = 16;    // persistent warps per SM
+
+// Dynamic shared memory above 48 KB has to be asked for (on every device; it costs the host under a microsecond).
+template <typename K>
+int room_for(K kernel, size_t bytes) {
+  if (bytes <= 40 * 1024) return F16_OK;          // with what a kernel declares itself
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess ? F16_OK : F16_ERR_CUDA;
+}
+
+// f(V, E, LANES) for a plan, as integral constants.
+template <typename T, typename F>
+void with_plan(const Plan& p, F f) {
+  constexpr int VW = 16 / sizeof(T);
+  const auto with = [&](auto v, auto e, auto lanes) { f(v, e, lanes); };
+  const auto lanes_of = [&](auto v, auto e) {
+    if (p.lanes > 256) with(v, e, std::integral_constant<int, 512>());
+    else if (p.lanes > 128) with(v, e, std::integral_constant<int, 256>());
+    else if (p.lanes > 64) with(v, e, std::integral_constant<int, 128>());
+    else if (p.lanes > 32) with(v, e, std::integral_constant<int, 64>());
+    else if (p.lanes == 32) with(v, e, std::integral_constant<int, 32>());
+    else with(v, e, std::integral_constant<int, 0>());
+  };
+  const std::integral_constant<int, MOST> all;
+  const std::integral_constant<int, MOST / 2> half;
+  if (p.v == VW) lanes_of(std::integral_constant<int, VW>(), all);
+  else if (p.v == 2 && p.e == MOST) with(std::integral_constant<int, 2>(), all, std::integral_constant<int, 512>());
+  else if (p.v == 2) lanes_of(std::integral_constant<int, 2>(), half);
+  else if (p.e == MOST) with(std::integral_constant<int, 1>(), all, std::integral_constant<int, 512>());
+  else lanes_of(std::integral_constant<int, 1>(), half);
+}
 
 template <typename T>
 int forward(const T* x, int64_t rows, int cols, int64_t ldx, Weights wb, float eps, T* y, int64_t ldy, float* mean,
@@ -387,33 +565,20 @@ int forward(const T* x, int64_t rows, int cols, int64_t ldx, Weights wb, float e
   const void* ptrs[2] = {x, y};
   const int64_t lds[2] = {ldx, ldy};
   const Plan p = plan_for(cols, vec_for(cols, sizeof(T), ptrs, lds, 2));
-  if (!p.nv) {
+  if (!p.lanes) {
     const int64_t grid = rows < 2 * sm_count() ? rows : 2 * sm_count();
     k_ln_fwd_wide<T><<<(unsigned)grid, WIDE, 0, st>>>(x, ldx, rows, cols, wb, eps, y, ldy, mean, rstd);
     return launch_status();
   }
   const unsigned grid = (unsigned)grid_rows(rows, p, FWD_WARPS);
-  const auto go = [&](auto k) {
-    k<<<grid, p.threads, 0, st>>>(x, ldx, rows, cols, wb, eps, y, ldy, mean, rstd, p.lanes);
-  };
-  constexpr int VW = 16 / sizeof(T);
-  if (p.v == VW) {
-    if (p.nv == 1) go(k_ln_fwd<T, VW, 1>);
-    else if (p.nv == 2) go(k_ln_fwd<T, VW, 2>);
-    else if constexpr (VW == 4) go(k_ln_fwd<T, VW, 4>);
-  } else if (p.v == 2) {
-    if (p.nv == 1) go(k_ln_fwd<T, 2, 1>);
-    else if (p.nv == 2) go(k_ln_fwd<T, 2, 2>);
-    else if (p.nv == 4) go(k_ln_fwd<T, 2, 4>);
-    else go(k_ln_fwd<T, 2, 8>);
-  } else {
-    if (p.nv == 1) go(k_ln_fwd<T, 1, 1>);
-    else if (p.nv == 2) go(k_ln_fwd<T, 1, 2>);
-    else if (p.nv == 4) go(k_ln_fwd<T, 1, 4>);
-    else if (p.nv == 8) go(k_ln_fwd<T, 1, 8>);
-    else go(k_ln_fwd<T, 1, 16>);
-  }
-  return launch_status();
+  int rc = F16_OK;
+  with_plan<T>(p, [&](auto v, auto e, auto lanes) {
+    const auto k = k_ln_fwd<T, v(), e(), lanes()>;
+    const size_t smem = Ring<T, v(), e(), 1>::bytes(p.threads);
+    rc = room_for(k, smem);
+    if (rc == F16_OK) k<<<grid, p.threads, smem, st>>>(x, ldx, rows, cols, wb, eps, y, ldy, mean, rstd, p.lanes);
+  });
+  return rc != F16_OK ? rc : launch_status();
 }
 
 template <typename T>
@@ -423,35 +588,23 @@ int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, in
   const void* ptrs[3] = {dy, x, dx};
   const int64_t lds[3] = {ldg, ldx, ldd};
   const Plan p = plan_for(cols, vec_for(cols, sizeof(T), ptrs, lds, 3));
-  int64_t grid = p.nv ? grid_rows(rows, p, BWD_WARPS) : (rows < sm_count() ? rows : sm_count());
+  int64_t grid = p.lanes ? grid_rows(rows, p, BWD_WARPS) : (rows < sm_count() ? rows : sm_count());
   if (part && grid > part_floats / (2 * (int64_t)cols)) grid = part_floats / (2 * (int64_t)cols);
   if (grid < 1) return F16_ERR_ARG;
-  if (!p.nv) {
+  int rc = F16_OK;
+  if (!p.lanes) {
     k_ln_bwd_wide<T><<<(unsigned)grid, WIDE, 0, st>>>(dy, ldg, x, ldx, rows, cols, wb, mean, rstd, dx, ldd, part);
   } else {
-    const size_t smem = part && p.threads > p.lanes ? 2 * (size_t)cols * sizeof(float) : 0;
-    const auto go = [&](auto k) {
-      k<<<(unsigned)grid, p.threads, smem, st>>>(dy, ldg, x, ldx, rows, cols, wb, mean, rstd, dx, ldd, part, p.lanes);
-    };
-    constexpr int VW = 16 / sizeof(T);
-    if (p.v == VW) {
-      if (p.nv == 1) go(k_ln_bwd<T, VW, 1>);
-      else if (p.nv == 2) go(k_ln_bwd<T, VW, 2>);
-      else if constexpr (VW == 4) go(k_ln_bwd<T, VW, 4>);
-    } else if (p.v == 2) {
-      if (p.nv == 1) go(k_ln_bwd<T, 2, 1>);
-      else if (p.nv == 2) go(k_ln_bwd<T, 2, 2>);
-      else if (p.nv == 4) go(k_ln_bwd<T, 2, 4>);
-      else go(k_ln_bwd<T, 2, 8>);
-    } else {
-      if (p.nv == 1) go(k_ln_bwd<T, 1, 1>);
-      else if (p.nv == 2) go(k_ln_bwd<T, 1, 2>);
-      else if (p.nv == 4) go(k_ln_bwd<T, 1, 4>);
-      else if (p.nv == 8) go(k_ln_bwd<T, 1, 8>);
-      else go(k_ln_bwd<T, 1, 16>);
-    }
+    with_plan<T>(p, [&](auto v, auto e, auto lanes) {
+      const auto k = k_ln_bwd<T, v(), e(), lanes()>;
+      const size_t ring = Ring<T, v(), e(), 2>::bytes(p.threads), sums = p.lanes <= 32 ? 2 * (size_t)cols * sizeof(float) : 0;
+      const size_t smem = ring > sums ? ring : sums;
+      rc = room_for(k, smem);
+      if (rc == F16_OK) k<<<(unsigned)grid, p.threads, smem, st>>>(dy, ldg, x, ldx, rows, cols, wb, mean, rstd, dx, ldd, part, p.lanes);
+    });
+    if (rc != F16_OK) return rc;
   }
-  const int rc = launch_status();
+  rc = launch_status();
   if (rc != F16_OK || !part) return rc;
   k_ln_wgrad<<<(unsigned)((2 * (int64_t)cols + 31) / 32), dim3(32, 32), 0, st>>>(part, (int)grid, cols, dw, db, wb.dtype);
   return launch_status();
@@ -485,7 +638,7 @@ extern "C" int f16_layer_norm_fwd(const void* x, int64_t rows, int cols, int64_t
 
 extern "C" int64_t f16_layer_norm_scratch_floats(int64_t rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  // no block has less than one row, no SM more backward blocks than its warps allow
+  // no block has less than one row, no SM more backward blocks than its warps allow (two warps a block at least)
   const int64_t most = (int64_t)sm_count() * (ln::BWD_WARPS / 2);
   return 2 * (int64_t)cols * (rows < most ? rows : most);
 }
