@@ -345,35 +345,37 @@ __global__ void __launch_bounds__(32 * WARPS, FOLD_BLOCKS)
 }
 
 // What enters each segment, from the first on (BACK: the last): the maps of the segments before it, folded in
-// order.  32 channels a block, a warp on consecutive segments; `first`: what enters the first one, or NULL.
-constexpr int START_WARPS = 32, START_EACH = 16;      // warps of a block, segments of a warp at a time
+// order.  START_CHANNELS channels a block, each with a thread for every START_EACH consecutive segments, at
+// most START_PARTS of them at a time; `first`: what enters the first one, or NULL.
+constexpr int START_CHANNELS = 8, START_EACH = 16, START_PARTS = 32;
 template <bool BACK>
-__global__ void __launch_bounds__(32 * START_WARPS) k_scan_starts(const __grid_constant__ Shape sh, int64_t channels, const float* first) {
-  __shared__ float2 of_warp[START_WARPS][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+__global__ void __launch_bounds__(START_CHANNELS * START_PARTS)
+    k_scan_starts(const __grid_constant__ Shape sh, int64_t channels, const float* first) {
+  __shared__ float2 of_part[START_PARTS][START_CHANNELS];
+  const int mine = threadIdx.x / START_CHANNELS, parts = blockDim.x / START_CHANNELS, k = threadIdx.x % START_CHANNELS;
+  const int64_t c = (int64_t)blockIdx.x * START_CHANNELS + k;
   const bool live = c < channels;
   float h = first && live ? first[c] : 0.0f;
-  for (int base = 0; base < sh.segments; base += START_WARPS * START_EACH) {
-    const int begin = base + warp * START_EACH;
+  for (int base = 0; base < sh.segments; base += parts * START_EACH) {
+    const int begin = base + mine * START_EACH;
     const auto at = [&](int i) { return (BACK ? sh.segments - 1 - i : i) * channels + c; };
     float2 m[START_EACH], all = make_float2(1.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < START_EACH; i++) m[i] = live && begin + i < sh.segments ? sh.maps[at(begin + i)] : make_float2(1.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < START_EACH; i++) all = then(all, m[i]);
-    of_warp[warp][lane] = all;
+    of_part[mine][k] = all;
     __syncthreads();
-    float mine = h;
+    float enter = h;
 #pragma unroll 8
-    for (int w = 0; w < START_WARPS; w++) {
-      if (w == warp) mine = h;
-      h = pass_through(of_warp[w][lane], h);
+    for (int w = 0; w < parts; w++) {
+      if (w == mine) enter = h;
+      h = pass_through(of_part[w][k], h);
     }
 #pragma unroll
     for (int i = 0; i < START_EACH; i++) {
-      if (live && begin + i < sh.segments) sh.starts[at(begin + i)] = mine;
-      mine = pass_through(m[i], mine);
+      if (live && begin + i < sh.segments) sh.starts[at(begin + i)] = enter;
+      enter = pass_through(m[i], enter);
     }
     __syncthreads();
   }
@@ -626,16 +628,21 @@ int run(const Args& p, bool grad, cudaStream_t st) {
     s.segments = 1;
     s.length = (int)((p.steps + CHUNK - 1) / CHUNK * CHUNK);
   }
-  const int64_t grid = (s.groups * s.segments + WARPS - 1) / WARPS, starts = (channels + 31) / 32;
+  const int64_t grid = (s.groups * s.segments + WARPS - 1) / WARPS, starts = (channels + START_CHANNELS - 1) / START_CHANNELS;
   if (grid > 0x7fffffff) return F16_ERR_TOO_LARGE;
   const unsigned blocks = (unsigned)grid, threads = 32 * WARPS;
+  // whole warps of parts, none for segments that are not there
+  int parts = (s.segments + START_EACH - 1) / START_EACH;
+  parts = parts > START_PARTS ? START_PARTS : (parts + 3) / 4 * 4;
+  const int start_threads = parts * START_CHANNELS;
+  if (s.maps && starts > 0x7fffffff) return F16_ERR_TOO_LARGE;
   if (s.maps) {
     if (grad) {
       k_scan_fold<T, V, GATED, true><<<blocks, threads, 0, st>>>(p, s);
-      k_scan_starts<true><<<(unsigned)starts, 32 * START_WARPS, 0, st>>>(s, channels, p.dhn);
+      k_scan_starts<true><<<(unsigned)starts, start_threads, 0, st>>>(s, channels, p.dhn);
     } else {
       k_scan_fold<T, V, GATED, false><<<blocks, threads, 0, st>>>(p, s);
-      k_scan_starts<false><<<(unsigned)starts, 32 * START_WARPS, 0, st>>>(s, channels, p.h0);
+      k_scan_starts<false><<<(unsigned)starts, start_threads, 0, st>>>(s, channels, p.h0);
     }
   }
   if (grad) k_scan_grad<T, V, GATED><<<blocks, threads, 0, st>>>(p, s);

@@ -30,7 +30,7 @@ def _row_stride(x):
 
 def _forward(x, rows, weight, bias, eps, stats):
     n, dim = rows.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     if n:
         wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
         at = stats.data_ptr() if stats is not None else None
@@ -47,7 +47,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows = _rows(x)
-        stats = torch.empty(2, rows.shape[0], dtype=torch.float32, device=x.device)
+        stats = x.new_empty(2, rows.shape[0], dtype=torch.float32)
         ctx.wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
         ctx.save_for_backward(rows, weight, stats)
         return _forward(x, rows, weight, bias, eps, stats)
@@ -60,16 +60,16 @@ class _LayerNorm(torch.autograd.Function):
         n, dim = x.shape
         shape = dy.shape
         dy = _rows(dy)
-        dx = torch.empty(shape, dtype=x.dtype, device=x.device) if need_x else None
+        dx = x.new_empty(shape) if need_x else None
         if not n:
             zero = torch.zeros(dim, dtype=ctx.wdtype, device=x.device) if need_w or need_b else None
             return dx, zero if need_w else None, zero.clone() if need_b else None, None
-        dw = torch.empty(dim, dtype=ctx.wdtype, device=x.device) if need_w else None
-        db = torch.empty(dim, dtype=ctx.wdtype, device=x.device) if need_b else None
+        dw = x.new_empty(dim, dtype=ctx.wdtype) if need_w else None
+        db = x.new_empty(dim, dtype=ctx.wdtype) if need_b else None
         lib = _lib.load()
         with _lib.on_device(x):
             room = lib.f16_layer_norm_scratch_floats(n, dim) if need_w or need_b else 0
-            scratch = torch.empty(room, dtype=torch.float32, device=x.device) if room else None
+            scratch = x.new_empty(room, dtype=torch.float32) if room else None
             at = stats.data_ptr()
             _lib.check(lib.f16_layer_norm_bwd(
                 dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), n, dim, _lib.DTYPES[x.dtype],

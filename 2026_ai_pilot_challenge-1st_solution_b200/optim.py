@@ -30,7 +30,7 @@ BLOCK = 256                     # F16_ADAMW_BLOCK: values that share a scale
 LAUNCH_TENSORS, LAUNCH_PARTIALS = 720, 592      # tensors of one launch, and the partial sums it may write
 
 
-_grad, _layout, _dtype = (operator.attrgetter(name) for name in ("grad", "layout", "dtype"))
+_grad, _nbytes, _dtype = (operator.attrgetter(name) for name in ("grad", "nbytes", "dtype"))
 _numel, _device, _contiguous, _address = (torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous,
                                           torch.Tensor.data_ptr)
 
@@ -97,13 +97,14 @@ class _Bucket:
             if not live:
                 return None
             params, grads, numels = [params[i] for i in live], [grads[i] for i in live], [numels[i] for i in live]
-        both = params + grads
-        if set(map(_layout, grads)) != {torch.strided}:
-            raise RuntimeError("AdamW does not take sparse gradients")
-        if (list(map(_numel, both)) != numels + numels or set(map(_dtype, both)) != {self.dtype}
-                or set(map(_device, both)) != {self.device.index} or not all(map(_contiguous, params))):
+        # torch lets a gradient differ from its parameter only where the parameter's storage was swapped after
+        # the gradient was set; sizes in bytes and devices are what a launch relies on
+        size = self.dtype.itemsize
+        if (list(map(_numel, params)) != numels or set(map(_dtype, params)) != {self.dtype}
+                or list(map(_nbytes, grads)) != [size * n for n in numels]
+                or set(map(_device, params + grads)) != {self.device.index} or not all(map(_contiguous, params))):
             raise RuntimeError("a parameter's or a gradient's size, type, device or layout is not what it was when the "
-                               "optimiser was made")
+                               "optimiser was made (sparse gradients are not taken)")
         if not all(map(_contiguous, grads)):
             grads = [g.detach().contiguous() for g in grads]
         n = len(live)

@@ -49,7 +49,7 @@ def _at(t):
 def _scratch(lib, x):
     """(buffer, values in it) for the segments of a scan with few channels, or (None, 0)."""
     n = lib.f16_scan_scratch_floats(*x.shape)
-    return (torch.empty(n, dtype=torch.float32, device=x.device) if n else None), n
+    return (x.new_empty(n, dtype=torch.float32) if n else None), n
 
 
 def _args(gate, x, h0, reset, lengths, gated, h, hn, saved, scratch, dh=None, dhn=None, dgate=None, dx=None, dh0=None):
@@ -64,14 +64,14 @@ def _forward(gate, x, h0, reset, lengths, gated, keep):
     """(h, hn, the states that the backward pass needs if ``keep``); gate and x with unit stride along dim."""
     steps, batch, dim = x.shape
     h = _like(x)
-    hn = torch.empty(batch, dim, dtype=torch.float32, device=x.device)
+    hn = x.new_empty(batch, dim, dtype=torch.float32)
     saved = None
     if not x.numel():
         hn.zero_() if h0 is None else hn.copy_(h0)
     else:
         lib = _lib.load()
         if keep:
-            saved = torch.empty(lib.f16_scan_saved_floats(steps, batch, dim), dtype=torch.float32, device=x.device)
+            saved = x.new_empty(lib.f16_scan_saved_floats(steps, batch, dim), dtype=torch.float32)
         with _lib.on_device(x):
             scratch = _scratch(lib, x)
             a = _args(gate, x, h0, reset, lengths, gated, h, hn, saved, scratch)
@@ -98,7 +98,7 @@ class _Scan(torch.autograd.Function):
         need_gate, need_x, need_h0 = ctx.needs_input_grad[:3]
         dgate = _like(gate) if need_gate else None
         dx = _like(x) if need_x else None
-        dh0 = torch.empty(x.shape[1:], dtype=torch.float32, device=x.device) if need_h0 else None
+        dh0 = x.new_empty(x.shape[1:], dtype=torch.float32) if need_h0 else None
         if not x.numel():
             if dh0 is not None:
                 dh0.zero_() if dhn is None else dh0.copy_(dhn)
@@ -155,7 +155,7 @@ def _step(gate, x, state, reset, out, gated, name):
     _lib.checked(gate, (x.dtype,), shape, "gate" if gated else "coefficients", x)
     _lib.checked(state, _F32, shape, "state", x)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
     else:
         _lib.checked(out, (x.dtype,), shape, "output", x)
     if reset is not None:
