@@ -19,11 +19,11 @@ namespace ln {
 
 constexpr int BLOCK = 256;          // threads of a block whose rows take a warp or less
 constexpr int MAX_LANES = 512;      // threads of a row: 128 registers each
-// Values of a row in one thread: 16, or 8 where loads are narrower than 16 bytes and the row's threads suffice.
+// Most values of a row in one thread.  16-byte loads always take so many; with narrower ones a thread of a
+// row that a warp holds takes 2, 4 or 8, of one that a block holds 8, as long as its threads suffice.
 constexpr int MOST = 16;
-constexpr int WIDE = 1024;          // threads of a block on a row too wide for registers
-
-constexpr int threads_of(int lanes) { return lanes > 32 ? lanes : BLOCK; }
+constexpr int MAX_COLS = 1 << 29;   // column indexes are 32-bit
+constexpr int WIDE = 512, WIDE_PER_SM = 3;      // threads of a block on a row too wide for registers, blocks on an SM
 
 struct Weights {
   const void* w;
@@ -36,6 +36,38 @@ __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i
   if (dtype == F16_DTYPE_BF16) return to_f32(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
   return to_f32(reinterpret_cast<const __half*>(p)[i]);
 }
+// V of them from i on, a multiple of V: 16 bytes a load where the weights are aligned so.
+template <int V, typename W>
+__device__ __forceinline__ void load_weights_of(float (&w)[V], const W* p) {
+  constexpr int N = 16 / (int)sizeof(W);
+  if constexpr (V % 4 == 0) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      constexpr int M = V < N ? V : N;
+#pragma unroll
+      for (int j = 0; j < V; j += M) {
+        const Vec<W, M> v = load_vec_nc<W, M>(p + j);
+#pragma unroll
+        for (int k = 0; k < M; k++) w[j + k] = to_f32(v.e[k]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < V; k++) w[k] = to_f32(p[k]);
+}
+template <int V>
+__device__ __forceinline__ void load_weights(float (&w)[V], const void* p, int dtype, int64_t i, float none) {
+  if (!p) {
+#pragma unroll
+    for (int k = 0; k < V; k++) w[k] = none;
+  } else if (dtype == F16_DTYPE_FP32) {
+    load_weights_of<V>(w, reinterpret_cast<const float*>(p) + i);
+  } else if (dtype == F16_DTYPE_BF16) {
+    load_weights_of<V>(w, reinterpret_cast<const __nv_bfloat16*>(p) + i);
+  } else {
+    load_weights_of<V>(w, reinterpret_cast<const __half*>(p) + i);
+  }
+}
 __device__ __forceinline__ void store_from_f32(void* p, int dtype, int64_t i, float v) {
   if (dtype == F16_DTYPE_FP32) reinterpret_cast<float*>(p)[i] = v;
   else if (dtype == F16_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
@@ -43,8 +75,9 @@ __device__ __forceinline__ void store_from_f32(void* p, int dtype, int64_t i, fl
 }
 
 // Sums over the threads of a row (xor shuffles: every thread gets the same bits).  LANES: 1 to 16 at run
-// time (0), 32, or a block of 64 to 512, whose warps meet in `red`; consecutive calls alternate its halves,
-// so one barrier a call is enough.
+// time (0), 32, or a whole block (ROW_BLOCK), whose warps meet in `red`; consecutive calls alternate its
+// halves, so one barrier a call is enough.
+constexpr int ROW_BLOCK = 64;
 template <int LANES, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*red)[N][32], int& half) {
   if constexpr (LANES == 0) {
@@ -57,19 +90,19 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int lanes, float (*red)[
 #pragma unroll
       for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(~0u, v[k], o);
   }
-  if constexpr (LANES > 32) {
-    constexpr int W = LANES / 32;
+  if constexpr (LANES == ROW_BLOCK) {
     float (*r)[32] = red[half];
     half ^= 1;
-    if ((threadIdx.x & 31) == 0) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) {
 #pragma unroll
       for (int k = 0; k < N; k++) r[k][threadIdx.x >> 5] = v[k];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < N; k++) v[k] = r[k][threadIdx.x & (W - 1)];
+    for (int k = 0; k < N; k++) v[k] = lane < warps ? r[k][lane] : 0.0f;
 #pragma unroll
-    for (int o = W / 2; o; o >>= 1)
+    for (int o = 16; o; o >>= 1)
 #pragma unroll
       for (int k = 0; k < N; k++) v[k] += __shfl_xor_sync(~0u, v[k], o);
   }
@@ -190,10 +223,10 @@ struct Place {
   unsigned there;
   bool full;                    // every thread of the row has all its values
   __device__ __forceinline__ Place(int cols, int run_lanes) {
-    lanes = LANES ? LANES : run_lanes;
-    lane = threadIdx.x & (lanes - 1);
-    group = LANES > 32 ? 0 : threadIdx.x / lanes;
-    per = LANES > 32 ? 1 : BLOCK / lanes;
+    lanes = LANES == 32 ? 32 : run_lanes;
+    lane = LANES == ROW_BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
+    group = LANES == ROW_BLOCK ? 0 : threadIdx.x / lanes;
+    per = LANES == ROW_BLOCK ? 1 : BLOCK / lanes;
     apart = lanes * V;
     there = 0;
 #pragma unroll
@@ -210,7 +243,7 @@ __device__ __forceinline__ float sum_of(const Two (&s)[2]) {
 }
 
 template <typename T, int V, int E, int LANES>
-__global__ void __launch_bounds__(threads_of(LANES), 768 / threads_of(LANES))
+__global__ void __maxnreg__(80)
     k_ln_fwd(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps, T* __restrict__ y,
              int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd, int lanes) {
   __shared__ float red[2][1][32];
@@ -229,7 +262,7 @@ __global__ void __launch_bounds__(threads_of(LANES), 768 / threads_of(LANES))
   const float inv = 1.0f / (float)cols;
   typedef Ring<T, V, E, 1> Rows;
   extern __shared__ __align__(16) unsigned char smem[];
-  Rows ring(smem, threads_of(LANES), at.there);
+  Rows ring(smem, LANES == ROW_BLOCK ? blockDim.x : BLOCK, at.there);
   const T* from[1] = {x + row * ldx + at.lane * V};
   int64_t ahead = row;
   const auto put = [&] {
@@ -287,7 +320,7 @@ __global__ void __launch_bounds__(threads_of(LANES), 768 / threads_of(LANES))
 // Backward of the rows of one block, and its columns' sums part[block][0][cols] (dw) and
 // part[block][1][cols] (db).  dx or part may be null.
 template <typename T, int V, int E, int LANES>
-__global__ void __launch_bounds__(threads_of(LANES), 512 / threads_of(LANES))
+__global__ void __maxnreg__(128)
     k_ln_bwd(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ x, int64_t ldx, int64_t rows, int cols,
              Weights wb, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
              int64_t ldd, float* __restrict__ part, int lanes) {
@@ -307,7 +340,7 @@ __global__ void __launch_bounds__(threads_of(LANES), 512 / threads_of(LANES))
   T* to = dx ? dx + row * ldd + at.lane * V : nullptr;
   const float inv = 1.0f / (float)cols;
   typedef Ring<T, V, E, 2> Rows;
-  Rows ring(smem, threads_of(LANES), at.there);
+  Rows ring(smem, LANES == ROW_BLOCK ? blockDim.x : BLOCK, at.there);
   const T* from[2] = {x + row * ldx + at.lane * V, dy + row * ldg + at.lane * V};
   int64_t ahead = row;
   const auto put = [&] {
@@ -364,7 +397,7 @@ __global__ void __launch_bounds__(threads_of(LANES), 512 / threads_of(LANES))
     split(aw[i], sw[2 * i], sw[2 * i + 1]);
     split(ab[i], sb[2 * i], sb[2 * i + 1]);
   }
-  if constexpr (LANES > 32) {
+  if constexpr (LANES == ROW_BLOCK) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const int c = at.column(e);
@@ -404,13 +437,13 @@ __global__ void __launch_bounds__(threads_of(LANES), 512 / threads_of(LANES))
 // The sum over a block of WIDE threads.
 __device__ __forceinline__ float wide_sum(float v, float (*red)[1][32], int& half) {
   float t[1] = {v};
-  row_sums<WIDE, 1>(t, WIDE, red, half);
+  row_sums<ROW_BLOCK, 1>(t, WIDE, red, half);
   return t[0];
 }
 
-// Rows too wide for a block's registers: a block a row, read again for each of the three passes (the
-// second and third hit L2).
-template <typename T>
+// Rows too wide for a block's registers: a block a row, V values a load, read again for each of the passes
+// (the second and third hit L1 and L2).
+template <typename T, int V>
 __global__ void __launch_bounds__(WIDE)
     k_ln_fwd_wide(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps,
                   T* __restrict__ y, int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd) {
@@ -420,66 +453,116 @@ __global__ void __launch_bounds__(WIDE)
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
     float s = 0.0f, q = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += WIDE) s += to_f32(xr[c]);
+    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+      const Vec<T, V> v = load_vec<T, V>(xr + c);
+#pragma unroll
+      for (int k = 0; k < V; k++) s += to_f32(v.e[k]);
+    }
     const float mu = wide_sum(s, red, half) * inv;
-    for (int c = threadIdx.x; c < cols; c += WIDE) {
-      const float d = to_f32(xr[c]) - mu;
-      q = fmaf(d, d, q);
+    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+      const Vec<T, V> v = load_vec<T, V>(xr + c);
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float d = to_f32(v.e[k]) - mu;
+        q = fmaf(d, d, q);
+      }
     }
     const float r = rsqrtf(wide_sum(q, red, half) * inv + eps);
     if (threadIdx.x == 0 && mean) {
       mean[row] = mu;
       rstd[row] = r;
     }
-    for (int c = threadIdx.x; c < cols; c += WIDE) {
-      const float w = wb.w ? load_as_f32(wb.w, wb.dtype, c) : 1.0f, b = wb.b ? load_as_f32(wb.b, wb.dtype, c) : 0.0f;
-      y[row * ldy + c] = from_f32<T>(fmaf((to_f32(xr[c]) - mu) * r, w, b));
+    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+      Vec<T, V> v = load_vec<T, V>(xr + c);
+      float w[V], b[V];
+      load_weights<V>(w, wb.w, wb.dtype, c, 1.0f);
+      load_weights<V>(b, wb.b, wb.dtype, c, 0.0f);
+#pragma unroll
+      for (int k = 0; k < V; k++) v.e[k] = from_f32<T>(fmaf((to_f32(v.e[k]) - mu) * r, w[k], b[k]));
+      store_vec<T, V>(y + row * ldy + c, v);
     }
   }
 }
 
-// Its backward: every thread keeps its columns' sums in the block's row of `part`.
-template <typename T>
+// Their dx; the sums over rows are k_ln_cols's.
+template <typename T, int V>
 __global__ void __launch_bounds__(WIDE)
     k_ln_bwd_wide(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ x, int64_t ldx, int64_t rows, int cols,
                   Weights wb, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
-                  int64_t ldd, float* part) {
+                  int64_t ldd) {
   __shared__ float red[2][1][32];
   int half = 0;
   const float inv = 1.0f / (float)cols;
-  float* out = part ? part + (int64_t)blockIdx.x * 2 * cols : nullptr;
-  bool first = true;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, first = false) {
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const float mu = mean[row], r = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += WIDE) {
-      const float d = to_f32(dy[row * ldg + c]), xh = (to_f32(x[row * ldx + c]) - mu) * r;
-      const float g = wb.w ? d * load_as_f32(wb.w, wb.dtype, c) : d;
-      s1 += g;
-      s2 = fmaf(g, xh, s2);
-      if (out) {
-        out[c] = first ? d * xh : fmaf(d, xh, out[c]);
-        out[cols + c] = first ? d : out[cols + c] + d;
+    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+      const Vec<T, V> xv = load_vec<T, V>(x + row * ldx + c), gv = load_vec<T, V>(dy + row * ldg + c);
+      float w[V];
+      load_weights<V>(w, wb.w, wb.dtype, c, 1.0f);
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float xh = (to_f32(xv.e[k]) - mu) * r, g = to_f32(gv.e[k]) * w[k];
+        s1 += g;
+        s2 = fmaf(g, xh, s2);
       }
     }
-    if (!dx) continue;
     const float m1 = wide_sum(s1, red, half) * inv, m2 = wide_sum(s2, red, half) * inv;
-    for (int c = threadIdx.x; c < cols; c += WIDE) {
-      const float xh = (to_f32(x[row * ldx + c]) - mu) * r;
-      const float g = to_f32(dy[row * ldg + c]) * (wb.w ? load_as_f32(wb.w, wb.dtype, c) : 1.0f);
-      dx[row * ldd + c] = from_f32<T>(r * (g - m1 - xh * m2));
+    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+      const Vec<T, V> xv = load_vec<T, V>(x + row * ldx + c), gv = load_vec<T, V>(dy + row * ldg + c);
+      Vec<T, V> o;
+      float w[V];
+      load_weights<V>(w, wb.w, wb.dtype, c, 1.0f);
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float xh = (to_f32(xv.e[k]) - mu) * r, g = to_f32(gv.e[k]) * w[k];
+        o.e[k] = from_f32<T>(r * (g - m1 - xh * m2));
+      }
+      store_vec<T, V>(dx + row * ldd + c, o);
     }
+  }
+}
+
+// Column sums part[slice][0][cols] (dw) and part[slice][1][cols] (db) of wide rows: a thread has V columns
+// (blockIdx.x) of the rows of a slice (blockIdx.y).
+constexpr int COLS = 256;
+template <typename T, int V>
+__global__ void __launch_bounds__(COLS)
+    k_ln_cols(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ x, int64_t ldx, int64_t rows, int cols,
+              const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part) {
+  const int64_t per = (rows + gridDim.y - 1) / gridDim.y, first = blockIdx.y * per, end = first + per < rows ? first + per : rows;
+  const int64_t c = ((int64_t)blockIdx.x * COLS + threadIdx.x) * V;
+  if (c >= cols) return;
+  float aw[V], ab[V];
+#pragma unroll
+  for (int k = 0; k < V; k++) aw[k] = ab[k] = 0.0f;
+#pragma unroll 4
+  for (int64_t row = first; row < end; row++) {
+    const Vec<T, V> xv = load_vec_nc<T, V>(x + row * ldx + c), gv = load_vec_nc<T, V>(dy + row * ldg + c);
+    const float mu = mean[row], r = rstd[row];
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+      const float d = to_f32(gv.e[k]);
+      aw[k] = fmaf(d, (to_f32(xv.e[k]) - mu) * r, aw[k]);
+      ab[k] += d;
+    }
+  }
+  float* out = part + blockIdx.y * 2 * (int64_t)cols + c;
+#pragma unroll
+  for (int k = 0; k < V; k++) {
+    out[k] = aw[k];
+    out[cols + k] = ab[k];
   }
 }
 
 // dw and db from the blocks' partial sums: 32 columns a block, 32 threads a column, in a fixed order.
-__global__ void __launch_bounds__(1024) k_ln_wgrad(const float* __restrict__ part, int nblk, int cols, void* dw, void* db,
+__global__ void __launch_bounds__(1024) k_ln_wgrad(const float* __restrict__ part, int64_t nblk, int cols, void* dw, void* db,
                                                    int dtype) {
   __shared__ float s[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float v = 0.0f;
   if (c < 2 * cols)
-    for (int r = threadIdx.y; r < nblk; r += 32) v += part[(int64_t)r * 2 * cols + c];
+    for (int64_t r = threadIdx.y; r < nblk; r += 32) v += part[r * 2 * cols + c];
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   v = s[threadIdx.x][threadIdx.y];
@@ -494,19 +577,21 @@ __global__ void __launch_bounds__(1024) k_ln_wgrad(const float* __restrict__ par
   }
 }
 
-// How a row is spread: v values a load, e values a thread, `lanes` threads a row -- a power of two, the
-// fewest that hold it; 0: the wide kernels.
+// How a row is spread: v values a load, e values a thread, `lanes` threads a row -- a power of two up to 32, or
+// whole warps, the fewest that hold it; 0: the wide kernels.
 struct Plan {
   int v, e, lanes, threads;
 };
 
 inline Plan plan_for(int cols, int v) {
-  Plan p = {v, v > 2 || cols > MOST / 2 * MAX_LANES ? MOST : MOST / 2, 1, BLOCK};
-  while (p.lanes * p.e < cols) p.lanes <<= 1;
-  // one value a load: a warp's request should cover 32 neighbours before a thread takes many values
-  if (v == 1)
-    while (p.lanes < 32 && p.lanes < cols) p.lanes <<= 1;
-  if (p.lanes > MAX_LANES) p.lanes = 0;
+  Plan p = {v, MOST, 1, BLOCK};
+  if (v <= 2) {
+    p.e = 2 * v;
+    while (p.e < MOST / 2 && p.e * 32 < cols) p.e *= 2;
+    if (cols > MOST / 2 * MAX_LANES) p.e = MOST;
+  }
+  while (p.lanes < 32 && p.lanes * p.e < cols) p.lanes <<= 1;
+  if (p.lanes * p.e < cols) p.lanes = cols > p.e * MAX_LANES ? 0 : (cols + 32 * p.e - 1) / (32 * p.e) * 32;
   p.threads = p.lanes > 32 ? p.lanes : p.lanes ? BLOCK : WIDE;
   return p;
 }
@@ -538,25 +623,31 @@ int room_for(K kernel, size_t bytes) {
 }
 
 // f(V, E, LANES) for a plan, as integral constants.
+template <int N> using Int = std::integral_constant<int, N>;
 template <typename T, typename F>
 void with_plan(const Plan& p, F f) {
   constexpr int VW = 16 / sizeof(T);
-  const auto with = [&](auto v, auto e, auto lanes) { f(v, e, lanes); };
-  const auto lanes_of = [&](auto v, auto e) {
-    if (p.lanes > 256) with(v, e, std::integral_constant<int, 512>());
-    else if (p.lanes > 128) with(v, e, std::integral_constant<int, 256>());
-    else if (p.lanes > 64) with(v, e, std::integral_constant<int, 128>());
-    else if (p.lanes > 32) with(v, e, std::integral_constant<int, 64>());
-    else if (p.lanes == 32) with(v, e, std::integral_constant<int, 32>());
-    else with(v, e, std::integral_constant<int, 0>());
-  };
-  const std::integral_constant<int, MOST> all;
-  const std::integral_constant<int, MOST / 2> half;
-  if (p.v == VW) lanes_of(std::integral_constant<int, VW>(), all);
-  else if (p.v == 2 && p.e == MOST) with(std::integral_constant<int, 2>(), all, std::integral_constant<int, 512>());
-  else if (p.v == 2) lanes_of(std::integral_constant<int, 2>(), half);
-  else if (p.e == MOST) with(std::integral_constant<int, 1>(), all, std::integral_constant<int, 512>());
-  else lanes_of(std::integral_constant<int, 1>(), half);
+  const auto of_warp = [&](auto v, auto e) { p.lanes == 32 ? f(v, e, Int<32>()) : f(v, e, Int<0>()); };
+  const auto of_any = [&](auto v, auto e) { p.lanes > 32 ? f(v, e, Int<ROW_BLOCK>()) : of_warp(v, e); };
+  if (p.v == VW) {
+    of_any(Int<VW>(), Int<MOST>());
+  } else if (p.v == 2) {
+    if (p.e == 4) of_warp(Int<2>(), Int<4>());
+    else if (p.e == 8) of_any(Int<2>(), Int<8>());
+    else f(Int<2>(), Int<MOST>(), Int<ROW_BLOCK>());
+  } else {
+    if (p.e == 2) of_warp(Int<1>(), Int<2>());
+    else if (p.e == 4) of_warp(Int<1>(), Int<4>());
+    else if (p.e == 8) of_any(Int<1>(), Int<8>());
+    else f(Int<1>(), Int<MOST>(), Int<ROW_BLOCK>());
+  }
+}
+
+// g(V) for rows too wide for registers.
+template <typename T, typename G>
+void with_loads(const Plan& p, G g) {
+  if (p.v == 16 / (int)sizeof(T)) g(Int<16 / (int)sizeof(T)>());
+  else g(Int<1>());
 }
 
 template <typename T>
@@ -566,8 +657,10 @@ int forward(const T* x, int64_t rows, int cols, int64_t ldx, Weights wb, float e
   const int64_t lds[2] = {ldx, ldy};
   const Plan p = plan_for(cols, vec_for(cols, sizeof(T), ptrs, lds, 2));
   if (!p.lanes) {
-    const int64_t grid = rows < 2 * sm_count() ? rows : 2 * sm_count();
-    k_ln_fwd_wide<T><<<(unsigned)grid, WIDE, 0, st>>>(x, ldx, rows, cols, wb, eps, y, ldy, mean, rstd);
+    const int64_t grid = rows < WIDE_PER_SM * sm_count() ? rows : WIDE_PER_SM * sm_count();
+    with_loads<T>(p, [&](auto v) {
+      k_ln_fwd_wide<T, v()><<<(unsigned)grid, WIDE, 0, st>>>(x, ldx, rows, cols, wb, eps, y, ldy, mean, rstd);
+    });
     return launch_status();
   }
   const unsigned grid = (unsigned)grid_rows(rows, p, FWD_WARPS);
@@ -588,13 +681,23 @@ int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, in
   const void* ptrs[3] = {dy, x, dx};
   const int64_t lds[3] = {ldg, ldx, ldd};
   const Plan p = plan_for(cols, vec_for(cols, sizeof(T), ptrs, lds, 3));
-  int64_t grid = p.lanes ? grid_rows(rows, p, BWD_WARPS) : (rows < sm_count() ? rows : sm_count());
-  if (part && grid > part_floats / (2 * (int64_t)cols)) grid = part_floats / (2 * (int64_t)cols);
-  if (grid < 1) return F16_ERR_ARG;
+  const int64_t room = part ? part_floats / (2 * (int64_t)cols) : 0;
+  int64_t grid = p.lanes ? grid_rows(rows, p, BWD_WARPS) : 0;
   int rc = F16_OK;
   if (!p.lanes) {
-    k_ln_bwd_wide<T><<<(unsigned)grid, WIDE, 0, st>>>(dy, ldg, x, ldx, rows, cols, wb, mean, rstd, dx, ldd, part);
+    with_loads<T>(p, [&](auto v) {
+      const int64_t blocks = rows < WIDE_PER_SM * sm_count() ? rows : WIDE_PER_SM * sm_count();
+      if (dx) k_ln_bwd_wide<T, v()><<<(unsigned)blocks, WIDE, 0, st>>>(dy, ldg, x, ldx, rows, cols, wb, mean, rstd, dx, ldd);
+      if (part) {
+        const int64_t tiles = (cols + COLS * v() - 1) / (COLS * v());
+        grid = (4 * sm_count() + tiles - 1) / tiles;
+        if (grid > rows) grid = rows;
+        if (grid > room) grid = room;
+        k_ln_cols<T, v()><<<dim3((unsigned)tiles, (unsigned)grid), COLS, 0, st>>>(dy, ldg, x, ldx, rows, cols, mean, rstd, part);
+      }
+    });
   } else {
+    if (part && grid > room) grid = room;
     with_plan<T>(p, [&](auto v, auto e, auto lanes) {
       const auto k = k_ln_bwd<T, v(), e(), lanes()>;
       const size_t ring = Ring<T, v(), e(), 2>::bytes(p.threads), sums = p.lanes <= 32 ? 2 * (size_t)cols * sizeof(float) : 0;
@@ -606,7 +709,7 @@ int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, in
   }
   rc = launch_status();
   if (rc != F16_OK || !part) return rc;
-  k_ln_wgrad<<<(unsigned)((2 * (int64_t)cols + 31) / 32), dim3(32, 32), 0, st>>>(part, (int)grid, cols, dw, db, wb.dtype);
+  k_ln_wgrad<<<(unsigned)((2 * (int64_t)cols + 31) / 32), dim3(32, 32), 0, st>>>(part, grid, cols, dw, db, wb.dtype);
   return launch_status();
 }
 
@@ -624,6 +727,7 @@ extern "C" int f16_layer_norm_fwd(const void* x, int64_t rows, int cols, int64_t
   if (!x || !y || rows <= 0 || cols <= 0 || ldx < 0 || ldy < cols || !ln::is_dtype(dtype) || !ln::is_dtype(wdtype) ||
       !mean != !rstd || !(eps >= 0.0))
     return F16_ERR_ARG;
+  if (cols > ln::MAX_COLS) return F16_ERR_TOO_LARGE;
   if (!aligned(x, ln::size_of(dtype)) || !aligned(y, ln::size_of(dtype)) || !aligned(weight, ln::size_of(wdtype)) ||
       !aligned(bias, ln::size_of(wdtype)))
     return F16_ERR_ALIGN;
@@ -650,6 +754,7 @@ extern "C" int f16_layer_norm_bwd(const void* dy, int64_t ldg, const void* x, in
   if (!dy || !x || !mean || !rstd || rows <= 0 || cols <= 0 || ldg < 0 || ldx < 0 || (dx && ldd < cols) ||
       !ln::is_dtype(dtype) || !ln::is_dtype(wdtype))
     return F16_ERR_ARG;
+  if (cols > ln::MAX_COLS) return F16_ERR_TOO_LARGE;
   const bool sums = dweight || dbias;
   if (!dx && !sums) return F16_OK;
   if (sums && (!scratch || scratch_floats < 2 * (int64_t)cols)) return F16_ERR_ARG;

@@ -16,6 +16,7 @@ from . import _lib
 
 
 _FLOATS = tuple(_lib.DTYPES)
+MAX_DIM = 2 ** 29
 
 
 def _rows(x):
@@ -83,8 +84,8 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (module docstring)."""
     _lib.checked(x, _FLOATS, None, "layer_norm input")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("layer_norm needs a last axis of at least one value")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
+        raise ValueError("layer_norm needs a last axis of 1 to 2^29 values")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     shape = x.shape[-1:]

@@ -525,7 +525,7 @@ int f16_categorical_bwd(const float* logits, int64_t ldz, int64_t M, int A, int 
 /* Layer norm of x [rows][cols] (row stride ldx, 0 allowed) over a row:
  * y = (x - mu) r w + b, mu the row's mean, r = 1 / sqrt(mean((x - mu)^2) + eps); weight / bias [cols]
  * of type wdtype or NULL (1 / 0).  mean / rstd [rows]: the statistics the backward pass reads (both
- * or neither).  Pointers are aligned to their type; 16-byte aligned rows run fastest. */
+ * or neither).  cols at most 2^29.  Pointers are aligned to their type; 16-byte aligned rows run fastest. */
 int f16_layer_norm_fwd(const void* x, int64_t rows, int cols, int64_t ldx, int dtype, const void* weight,
                        const void* bias, int wdtype, double eps, void* y, int64_t ldy, float* mean,
                        float* rstd, f16_stream_t stream);
