@@ -19,8 +19,9 @@ namespace ln {
 
 constexpr int BLOCK = 256;          // threads of a block whose rows take a warp or less
 constexpr int MAX_LANES = 512;      // threads of a row: 128 registers each
-// Most values of a row in one thread.  16-byte loads always take so many; with narrower ones a thread of a
-// row that a warp holds takes 2, 4 or 8, of one that a block holds 8, as long as its threads suffice.
+// Most values of a row in one thread.  16-byte loads take so many; with narrower ones a thread takes 8, of rows
+// up to 16 values 4 (500,000 x 33 fp16, forward + backward: 8 a thread 100 us, 4 142 us, 2 188 us;
+// 300,000 x 15 bf16: 30, 25 and 36 us), and 16 again where 8 do not suffice.
 constexpr int MOST = 16;
 constexpr int MAX_COLS = 1 << 29;   // column indexes are 32-bit
 constexpr int WIDE = 512, WIDE_PER_SM = 3;      // threads of a block on a row too wide for registers, blocks on an SM
@@ -31,11 +32,6 @@ struct Weights {
   int dtype;
 };
 
-__device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
-  if (dtype == F16_DTYPE_FP32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == F16_DTYPE_BF16) return to_f32(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return to_f32(reinterpret_cast<const __half*>(p)[i]);
-}
 // V of them from i on, a multiple of V: 16 bytes a load where the weights are aligned so.
 template <int V, typename W>
 __device__ __forceinline__ void load_weights_of(float (&w)[V], const W* p) {
@@ -237,6 +233,30 @@ struct Place {
   __device__ __forceinline__ int column(int e) const { return (e / V * lanes + lane) * V + e % V; }
 };
 
+// The thread's weights, or `none`: the branch on their type is outside the loop, so that all loads are under way
+// together (inside, a small call took 10 us of loads one after the other).
+template <int E, typename W, typename P>
+__device__ __forceinline__ void load_columns_of(Two (&w)[E / 2], const W* p, const P& at, int cols, float none) {
+  float f[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) f[e] = at.column(e) < cols ? to_f32(__ldg(p + at.column(e))) : none;
+#pragma unroll
+  for (int i = 0; i < E / 2; i++) w[i] = two(f[2 * i], f[2 * i + 1]);
+}
+template <int E, typename P>
+__device__ __forceinline__ void load_columns(Two (&w)[E / 2], const void* p, int dtype, const P& at, int cols, float none) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) w[i] = two(none);
+  } else if (dtype == F16_DTYPE_FP32) {
+    load_columns_of<E>(w, reinterpret_cast<const float*>(p), at, cols, none);
+  } else if (dtype == F16_DTYPE_BF16) {
+    load_columns_of<E>(w, reinterpret_cast<const __nv_bfloat16*>(p), at, cols, none);
+  } else {
+    load_columns_of<E>(w, reinterpret_cast<const __half*>(p), at, cols, none);
+  }
+}
+
 __device__ __forceinline__ float sum_of(const Two (&s)[2]) {
   const float2 f = split(s[0] + s[1]);
   return f.x + f.y;
@@ -251,12 +271,8 @@ __global__ void __maxnreg__(80)
   const Place<V, E, LANES> at(cols, lanes);
   const int64_t step = (int64_t)gridDim.x * at.per;
   Two w[E / 2], b[E / 2];
-#pragma unroll
-  for (int i = 0; i < E / 2; i++) {
-    const int c0 = at.column(2 * i), c1 = at.column(2 * i + 1);
-    w[i] = two(wb.w && c0 < cols ? load_as_f32(wb.w, wb.dtype, c0) : 1.0f, wb.w && c1 < cols ? load_as_f32(wb.w, wb.dtype, c1) : 1.0f);
-    b[i] = two(wb.b && c0 < cols ? load_as_f32(wb.b, wb.dtype, c0) : 0.0f, wb.b && c1 < cols ? load_as_f32(wb.b, wb.dtype, c1) : 0.0f);
-  }
+  load_columns<E>(w, wb.w, wb.dtype, at, cols, 1.0f);
+  load_columns<E>(b, wb.b, wb.dtype, at, cols, 0.0f);
   int64_t row = (int64_t)blockIdx.x * at.per + at.group;
   T* to = y + row * ldy + at.lane * V;
   const float inv = 1.0f / (float)cols;
@@ -330,12 +346,9 @@ __global__ void __maxnreg__(128)
   const Place<V, E, LANES> at(cols, lanes);
   const int64_t step = (int64_t)gridDim.x * at.per;
   Two w[E / 2], aw[E / 2], ab[E / 2];
+  load_columns<E>(w, wb.w, wb.dtype, at, cols, 1.0f);
 #pragma unroll
-  for (int i = 0; i < E / 2; i++) {
-    const int c0 = at.column(2 * i), c1 = at.column(2 * i + 1);
-    w[i] = two(wb.w && c0 < cols ? load_as_f32(wb.w, wb.dtype, c0) : 1.0f, wb.w && c1 < cols ? load_as_f32(wb.w, wb.dtype, c1) : 1.0f);
-    aw[i] = ab[i] = two(0.0f);
-  }
+  for (int i = 0; i < E / 2; i++) aw[i] = ab[i] = two(0.0f);
   int64_t row = (int64_t)blockIdx.x * at.per + at.group;
   T* to = dx ? dx + row * ldd + at.lane * V : nullptr;
   const float inv = 1.0f / (float)cols;
@@ -407,7 +420,7 @@ __global__ void __maxnreg__(128)
       }
     }
   } else {
-    // rows of one warp first (shuffles), then the warps in turn, in the ring's memory
+    // rows of one warp first (shuffles), then the warps' sums side by side in the ring's memory
     float* col_sum = reinterpret_cast<float*>(smem);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
@@ -417,20 +430,24 @@ __global__ void __maxnreg__(128)
         sw[e] += __shfl_xor_sync(~0u, sw[e], o);
         sb[e] += __shfl_xor_sync(~0u, sb[e], o);
       }
-    for (int turn = 0; turn < BLOCK / 32; turn++) {
-      if ((int)(threadIdx.x >> 5) == turn && (int)(threadIdx.x & 31) < at.lanes) {
+    if ((int)(threadIdx.x & 31) < at.lanes) {
+      float* mine = col_sum + (threadIdx.x >> 5) * 2 * cols;
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-          const int c = at.column(e);
-          if (c < cols) {
-            col_sum[c] = turn ? col_sum[c] + sw[e] : sw[e];
-            col_sum[cols + c] = turn ? col_sum[cols + c] + sb[e] : sb[e];
-          }
+      for (int e = 0; e < E; e++) {
+        const int c = at.column(e);
+        if (c < cols) {
+          mine[c] = sw[e];
+          mine[cols + c] = sb[e];
         }
       }
-      __syncthreads();
     }
-    for (int c = threadIdx.x; c < 2 * cols; c += BLOCK) out[c] = col_sum[c];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * cols; c += BLOCK) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < BLOCK / 32; w++) v += col_sum[w * 2 * cols + c];
+      out[c] = v;
+    }
   }
 }
 
@@ -586,9 +603,7 @@ struct Plan {
 inline Plan plan_for(int cols, int v) {
   Plan p = {v, MOST, 1, BLOCK};
   if (v <= 2) {
-    p.e = 2 * v;
-    while (p.e < MOST / 2 && p.e * 32 < cols) p.e *= 2;
-    if (cols > MOST / 2 * MAX_LANES) p.e = MOST;
+    p.e = cols <= 16 ? 4 : cols <= 8 * MAX_LANES ? 8 : MOST;
   }
   while (p.lanes < 32 && p.lanes * p.e < cols) p.lanes <<= 1;
   if (p.lanes * p.e < cols) p.lanes = cols > p.e * MAX_LANES ? 0 : (cols + 32 * p.e - 1) / (32 * p.e) * 32;
@@ -636,8 +651,7 @@ void with_plan(const Plan& p, F f) {
     else if (p.e == 8) of_any(Int<2>(), Int<8>());
     else f(Int<2>(), Int<MOST>(), Int<ROW_BLOCK>());
   } else {
-    if (p.e == 2) of_warp(Int<1>(), Int<2>());
-    else if (p.e == 4) of_warp(Int<1>(), Int<4>());
+    if (p.e == 4) of_warp(Int<1>(), Int<4>());
     else if (p.e == 8) of_any(Int<1>(), Int<8>());
     else f(Int<1>(), Int<MOST>(), Int<ROW_BLOCK>());
   }
@@ -700,7 +714,7 @@ int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, in
     if (part && grid > room) grid = room;
     with_plan<T>(p, [&](auto v, auto e, auto lanes) {
       const auto k = k_ln_bwd<T, v(), e(), lanes()>;
-      const size_t ring = Ring<T, v(), e(), 2>::bytes(p.threads), sums = p.lanes <= 32 ? 2 * (size_t)cols * sizeof(float) : 0;
+      const size_t ring = Ring<T, v(), e(), 2>::bytes(p.threads), sums = p.lanes <= 32 ? BLOCK / 32 * 2 * (size_t)cols * sizeof(float) : 0;
       const size_t smem = ring > sums ? ring : sums;
       rc = room_for(k, smem);
       if (rc == F16_OK) k<<<(unsigned)grid, p.threads, smem, st>>>(dy, ldg, x, ldx, rows, cols, wb, mean, rstd, dx, ldd, part, p.lanes);

@@ -35,8 +35,10 @@ constexpr int WARPS = 4;                  // of a block, each with channels (and
 // Blocks on an SM: 96, 128 and 80 registers a thread.
 constexpr int WALK_BLOCKS = 5, GRAD_BLOCKS = 4, FOLD_BLOCKS = 6;
 constexpr int MAX_SEGMENT = F16_SCAN_SEGMENT;      // steps whose coefficients' product is formed
-constexpr int WARPS_PER_SM = 64;          // in all: with less than half of them, time is cut
-static_assert(CHUNK <= 32, "resets of a chunk are bits of one word");
+// Time is cut where the channels give fewer than ENOUGH_PER_SM warps an SM, into so many segments that there
+// are WARPS_PER_SM, but no more than MAX_CUTS (k_scan_starts takes so many at once) while they are not too long.
+constexpr int ENOUGH_PER_SM = 12, WARPS_PER_SM = 64, MAX_CUTS = 1024;
+static_assert(CHUNK == 16, "the resets of a chunk are half a word");
 
 typedef f16_scan_args Args;
 
@@ -130,7 +132,9 @@ __device__ __forceinline__ float cut_mark() { return __int_as_float(0x7fffffff);
 struct Lane {
   int64_t b, d, c;      // sequence, feature, channel = b dim + d
   bool live;            // the channel exists
-  bool together;        // all channels of the warp belong to one sequence
+  int64_t first;        // the warp's first sequence, and how many it has channels of
+  int seqs;
+  bool together;        // one
   int len;              // the sequence's steps
 };
 
@@ -139,11 +143,12 @@ __device__ __forceinline__ Lane lane_of(const Args& p, int64_t c) {
   Lane l;
   l.c = c;
   l.live = c < p.batch * p.dim;
-  l.b = l.live ? c / p.dim : 0;
+  l.b = !l.live ? 0 : p.batch * p.dim <= 0xffffffffll ? (unsigned)c / (unsigned)p.dim : c / p.dim;
   l.d = l.live ? c - l.b * p.dim : 0;
-  const int64_t first = __shfl_sync(~0u, l.b, 0);
-  if (!l.live) l.b = first;
-  l.together = __all_sync(~0u, l.b == first);
+  l.first = __shfl_sync(~0u, l.b, 0);
+  if (!l.live) l.b = l.first;
+  l.seqs = (int)__reduce_max_sync(~0u, (unsigned)(l.b - l.first)) + 1;
+  l.together = l.seqs == 1;
   l.len = (int)p.steps;
   if (p.lengths) {
     const int64_t n = p.lengths[l.b];
@@ -158,22 +163,25 @@ __device__ __forceinline__ bool reset_at(const Args& p, int64_t b, int64_t t) {
                             : __ldg(reinterpret_cast<const float*>(p.reset) + i) != 0.0f;
 }
 
-// Bit i of resets_of: step t0 + i (of the n from t0 on) resets the lane's sequence.  Called by whole warps:
-// where a warp has one sequence its lanes read a step each, ahead of the time it is wanted (reset_ahead).
-__device__ __forceinline__ bool reset_ahead(const Args& p, const Lane& l, int t0) {
-  const int lane = threadIdx.x & 31, m = l.len - t0 < CHUNK ? l.len - t0 : CHUNK;
-  return p.reset && l.together && t0 >= 0 && lane < m && reset_at(p, l.b, t0 + lane);
+// Bit i of resets_of: step t0 + i of the CHUNK from t0 on resets the lane's sequence (past the sequence's length
+// it says nothing).  Called by whole warps, whose lanes read a step of a sequence each, two sequences at a
+// time; those of the first two ahead of the time they are wanted (reset_ahead).
+__device__ __forceinline__ bool reset_ahead(const Args& p, const Lane& l, int t0, int pair = 0) {
+  const int lane = threadIdx.x & 31, t = t0 + lane % CHUNK, seq = 2 * pair + lane / CHUNK;
+  return p.reset && t0 >= 0 && t < p.steps && seq < l.seqs && reset_at(p, l.first + seq, t);
 }
-__device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0, int n, bool ahead) {
+__device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0, bool ahead) {
   if (!p.reset) return 0;
-  if (l.together) return __ballot_sync(~0u, ahead);
-  unsigned m = 0;
-#pragma unroll 1
-  for (int i = 0; i < n; i++) m |= (unsigned)reset_at(p, l.b, t0 + i) << i;
-  return m;
+  unsigned word = __ballot_sync(~0u, ahead);
+  const int seq = (int)(l.b - l.first);
+  for (int pair = 1; 2 * pair < l.seqs; pair++) {
+    const unsigned next = __ballot_sync(~0u, reset_ahead(p, l, t0, pair));
+    if (seq >> 1 == pair) word = next;
+  }
+  return seq & 1 ? word >> CHUNK : word & ((1u << CHUNK) - 1);
 }
-__device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0, int n) {
-  return resets_of(p, l, t0, n, reset_ahead(p, l, t0));
+__device__ __forceinline__ unsigned resets_of(const Args& p, const Lane& l, int t0) {
+  return resets_of(p, l, t0, reset_ahead(p, l, t0));
 }
 
 // A tensor's element (t0, b, d), and how far it is to the next step's.
@@ -234,6 +242,7 @@ __device__ __forceinline__ void walk(const Vec<T, V> (&g)[CHUNK], const Vec<T, V
                                      int left, bool live, Line<T> out, P& h) {
 #pragma unroll
   for (int i = 0; i < CHUNK; i++) {
+    if (!PLAIN && i >= left) break;
     P a, b, k;
     step_of<GATED>(widen(g[i]), widen(x[i]), a, b, k);
     P o;
@@ -243,7 +252,7 @@ __device__ __forceinline__ void walk(const Vec<T, V> (&g)[CHUNK], const Vec<T, V
       h = pick(i < n, pick(cut >> i & 1, b, fma2(a, h, b)), h);
       o = pick(i < n, h, all_of<P>(0.0f));
     }
-    if (PLAIN || (live && i < left)) store_vec<T, V>(out.p, narrow<T, V>(o));
+    if (PLAIN || live) store_vec<T, V>(out.p, narrow<T, V>(o));
     advance(out.p, out.st);
   }
 }
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(32 * WARPS, WALK_BLOCKS) k_scan(const __grid_c
     Vec<T, V> g[CHUNK], x[CHUNK];
     load_chunk<T, V>(g, Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
     load_chunk<T, V>(x, Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
-    const unsigned cut = resets_of(p, l, t0, n);
+    const unsigned cut = resets_of(p, l, t0);
     const bool plain = all && __all_sync(~0u, cut == 0);
     if (p.saved) store_state<V>(p.saved + (int64_t)(t0 / CHUNK) * channels, h, l);
     const Line<T> out(p.h, p.h_t, p.h_b, l, t0);
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(32 * WARPS, FOLD_BLOCKS)
 #pragma unroll
       for (int i = 0; i < CHUNK; i++) x[i] = narrow<T, V>(all_of<P>(0.0f));
     }
-    const unsigned cut = resets_of(p, l, t0, n);
+    const unsigned cut = resets_of(p, l, t0);
     if (all && __all_sync(~0u, cut == 0)) fold<T, V, GATED, BACK, true>(g, x, 0, CHUNK, A, B);
     else fold<T, V, GATED, BACK, false>(g, x, cut, n, A, B);
   }
@@ -345,39 +354,44 @@ __global__ void __launch_bounds__(32 * WARPS, FOLD_BLOCKS)
 }
 
 // What enters each segment, from the first on (BACK: the last): the maps of the segments before it, folded in
-// order.  START_CHANNELS channels a block, each with a thread for every START_EACH consecutive segments, at
-// most START_PARTS of them at a time; `first`: what enters the first one, or NULL.
-constexpr int START_CHANNELS = 8, START_EACH = 16, START_PARTS = 32;
+// order.  A channel has `parts` threads, each with START_EACH consecutive segments at a time; `first`: what
+// enters the first one, or NULL.
+constexpr int START_THREADS = 256, START_EACH = 16, START_PARTS = 64;
 template <bool BACK>
-__global__ void __launch_bounds__(START_CHANNELS * START_PARTS)
-    k_scan_starts(const __grid_constant__ Shape sh, int64_t channels, const float* first) {
-  __shared__ float2 of_part[START_PARTS][START_CHANNELS];
-  const int mine = threadIdx.x / START_CHANNELS, parts = blockDim.x / START_CHANNELS, k = threadIdx.x % START_CHANNELS;
-  const int64_t c = (int64_t)blockIdx.x * START_CHANNELS + k;
+__global__ void __launch_bounds__(START_THREADS)
+    k_scan_starts(const __grid_constant__ Shape sh, int64_t channels, const float* first, int parts) {
+  __shared__ float2 of_part[START_THREADS];
+  const int block = START_THREADS / parts, mine = threadIdx.x / block, k = threadIdx.x % block;
+  const int64_t c = (int64_t)blockIdx.x * block + k;
   const bool live = c < channels;
   float h = first && live ? first[c] : 0.0f;
   for (int base = 0; base < sh.segments; base += parts * START_EACH) {
-    const int begin = base + mine * START_EACH;
+    const int begin = base + mine * START_EACH, count = sh.segments - begin < START_EACH ? sh.segments - begin : START_EACH;
     const auto at = [&](int i) { return (BACK ? sh.segments - 1 - i : i) * channels + c; };
     float2 m[START_EACH], all = make_float2(1.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < START_EACH; i++) m[i] = live && begin + i < sh.segments ? sh.maps[at(begin + i)] : make_float2(1.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < START_EACH; i++) all = then(all, m[i]);
-    of_part[mine][k] = all;
-    __syncthreads();
+    for (int i = 0; i < START_EACH; i++) m[i] = live && i < count ? sh.maps[at(begin + i)] : make_float2(1.0f, 0.0f);
     float enter = h;
+    if (parts > 1) {
+#pragma unroll
+      for (int i = 0; i < START_EACH; i++)
+        if (i < count) all = then(all, m[i]);
+      of_part[threadIdx.x] = all;
+      __syncthreads();
 #pragma unroll 8
-    for (int w = 0; w < parts; w++) {
-      if (w == mine) enter = h;
-      h = pass_through(of_part[w][k], h);
+      for (int w = 0; w < parts; w++) {
+        if (w == mine) enter = h;
+        h = pass_through(of_part[w * block + k], h);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < START_EACH; i++) {
-      if (live && begin + i < sh.segments) sh.starts[at(begin + i)] = enter;
-      enter = pass_through(m[i], enter);
-    }
-    __syncthreads();
+    for (int i = 0; i < START_EACH; i++)
+      if (i < count) {
+        if (live) sh.starts[at(begin + i)] = enter;
+        enter = pass_through(m[i], enter);
+      }
+    if (parts == 1) h = enter;
+    else __syncthreads();
   }
 }
 
@@ -478,6 +492,7 @@ __device__ __forceinline__ void walk_back(const I& in, int stage, unsigned cut, 
   P d[CHUNK];
 #pragma unroll
   for (int i = 0; i < CHUNK; i++) {
+    if (!PLAIN && i >= left) break;
     P a, b, k;
     const P xf = widen(in.x(stage, i));
     step_of<GATED>(widen(in.gate(stage, i)), xf, a, b, k);
@@ -489,11 +504,12 @@ __device__ __forceinline__ void walk_back(const I& in, int stage, unsigned cut, 
   asm volatile("" ::: "memory");        // the gates are read and worked out again, not kept
   // what reaches a step's state from the step after it is pass * carry
   P pass = all_of<P>(1.0f);
-  const int last = CHUNK - 1;
+  const int last = !PLAIN && left < CHUNK ? left - 1 : CHUNK - 1;
   dg.p += last * dg.st;
   dx.p += last * dx.st;
 #pragma unroll
   for (int i = CHUNK - 1; i >= 0; i--) {
+    if (!PLAIN && i >= left) continue;
     P a, b, k;
     step_of<GATED>(widen(in.gate(stage, i)), zero, a, b, k);
     const P G = fma2(pass, carry, in.dh(stage, i));
@@ -508,7 +524,7 @@ __device__ __forceinline__ void walk_back(const I& in, int stage, unsigned cut, 
       ox = pick(i < n, ox, zero);
       og = pick(i < n, og, zero);
     }
-    if (PLAIN || (live && i < left)) {
+    if (PLAIN || live) {
       if (want_g) store_vec<T, V>(dg.p, narrow<T, V>(og));
       if (want_x) store_vec<T, V>(dx.p, narrow<T, V>(ox));
     }
@@ -545,7 +561,7 @@ __global__ void __launch_bounds__(32 * WARPS, GRAD_BLOCKS)
   bool ahead = reset_ahead(p, l, first);
   for (int t0 = first; t0 >= begin; t0 -= CHUNK, h = h_next) {
     const int n = steps_of(l, t0), left = steps - t0, next = t0 - CHUNK;
-    const unsigned cut = resets_of(p, l, t0, n, ahead);
+    const unsigned cut = resets_of(p, l, t0, ahead);
     if constexpr (STAGED) in.fetch(p, l, stage ^ 1, next, next >= begin ? steps_of(l, next) : 0);
     h_next = saved_at(next);
     if (next >= begin) ahead = reset_ahead(p, l, next);
@@ -606,9 +622,10 @@ __global__ void __launch_bounds__(256)
 inline Shape shape_for(int64_t channels, int64_t steps, int v) {
   Shape s = {(channels + 32 * v - 1) / (32 * v), 1, (int)((steps + CHUNK - 1) / CHUNK * CHUNK), nullptr, nullptr};
   const int64_t want = (int64_t)sm_count() * WARPS_PER_SM, chunks = (steps + CHUNK - 1) / CHUNK;
-  if (s.groups * 2 > want || chunks < 2) return s;
+  if (s.groups >= (int64_t)sm_count() * ENOUGH_PER_SM || chunks < 2) return s;
   const int64_t cuts = (want + s.groups - 1) / s.groups;                 // at least two
   int64_t each = (chunks + cuts - 1) / cuts;                             // chunks of a segment
+  if (each < (chunks + MAX_CUTS - 1) / MAX_CUTS) each = (chunks + MAX_CUTS - 1) / MAX_CUTS;
   if (each > MAX_SEGMENT / CHUNK) each = MAX_SEGMENT / CHUNK;
   s.length = (int)each * CHUNK;
   s.segments = (int)((chunks + each - 1) / each);
@@ -628,21 +645,20 @@ int run(const Args& p, bool grad, cudaStream_t st) {
     s.segments = 1;
     s.length = (int)((p.steps + CHUNK - 1) / CHUNK * CHUNK);
   }
-  const int64_t grid = (s.groups * s.segments + WARPS - 1) / WARPS, starts = (channels + START_CHANNELS - 1) / START_CHANNELS;
+  const int64_t grid = (s.groups * s.segments + WARPS - 1) / WARPS;
   if (grid > 0x7fffffff) return F16_ERR_TOO_LARGE;
   const unsigned blocks = (unsigned)grid, threads = 32 * WARPS;
-  // whole warps of parts, none for segments that are not there
-  int parts = (s.segments + START_EACH - 1) / START_EACH;
-  parts = parts > START_PARTS ? START_PARTS : (parts + 3) / 4 * 4;
-  const int start_threads = parts * START_CHANNELS;
+  int parts = 1;
+  while (parts < START_PARTS && parts * START_EACH < s.segments) parts *= 2;
+  const int64_t starts = (channels + START_THREADS / parts - 1) / (START_THREADS / parts);
   if (s.maps && starts > 0x7fffffff) return F16_ERR_TOO_LARGE;
   if (s.maps) {
     if (grad) {
       k_scan_fold<T, V, GATED, true><<<blocks, threads, 0, st>>>(p, s);
-      k_scan_starts<true><<<(unsigned)starts, start_threads, 0, st>>>(s, channels, p.dhn);
+      k_scan_starts<true><<<(unsigned)starts, START_THREADS, 0, st>>>(s, channels, p.dhn, parts);
     } else {
       k_scan_fold<T, V, GATED, false><<<blocks, threads, 0, st>>>(p, s);
-      k_scan_starts<false><<<(unsigned)starts, start_threads, 0, st>>>(s, channels, p.h0);
+      k_scan_starts<false><<<(unsigned)starts, START_THREADS, 0, st>>>(s, channels, p.h0, parts);
     }
   }
   if (grad) k_scan_grad<T, V, GATED><<<blocks, threads, 0, st>>>(p, s);
