@@ -402,13 +402,21 @@ template <typename T, int V, bool STAGED> struct Inputs;
 template <typename T, int V> struct Inputs<T, V, true> {
   typedef unsigned Buffer[STAGES][3][CHUNK][32 * WARPS];
   unsigned* mine;
-  bool with_dh, rows;           // rows: a warp's row is 128 aligned bytes of one sequence in all three
-  __device__ __forceinline__ Inputs(Buffer& b, const Args& p, const Lane& l) : mine(&b[0][0][0][threadIdx.x]), with_dh(p.dh) {
+  bool with_dh;
+  // Rows by 16 bytes: a lane copies the four lanes' channels that begin at (b, d), of a sequence of `len` steps
+  // (0: there are none).  Where a unit lies in one sequence and is aligned in all inputs.
+  bool rows;
+  int b, d, len;
+  __device__ __forceinline__ Inputs(Buffer& buf, const Args& p, const Lane& l) : mine(&buf[0][0][0][threadIdx.x]), with_dh(p.dh) {
     const auto whole = [&](const void* q, int64_t st, int64_t sb) {
       return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ((st | sb) & (4 * V - 1)) == 0;
     };
-    rows = l.together && __all_sync(~0u, l.live) && p.dim % (4 * V) == 0 && whole(p.gate, p.gate_t, p.gate_b) &&
+    rows = p.dim % (4 * V) == 0 && p.dim <= 0x7fffffff && p.batch <= 0x7fffffff && whole(p.gate, p.gate_t, p.gate_b) &&
            whole(p.x, p.x_t, p.x_b) && (!with_dh || whole(p.dh, p.dh_t, p.dh_b));
+    const int first = (threadIdx.x & 7) * 4;
+    b = __shfl_sync(~0u, (int)l.b, first);
+    d = __shfl_sync(~0u, (int)l.d, first);
+    len = __shfl_sync(~0u, l.live ? l.len : 0, first);
   }
   __device__ __forceinline__ unsigned* at(int stage, int which, int i) const {
     return mine + ((stage * 3 + which) * CHUNK + i) * 32 * WARPS;
@@ -433,10 +441,9 @@ template <typename T, int V> struct Inputs<T, V, true> {
     }
   }
   // Eight lanes a row: 16 bytes each.
-  __device__ __forceinline__ void copy_rows(int stage, int which, const void* base, int64_t st, int64_t sb, const Lane& l,
-                                            int t0, int n) {
+  __device__ __forceinline__ void copy_rows(int stage, int which, const void* base, int64_t st, int64_t sb, int t0, int n) {
     const int lane = threadIdx.x & 31, row = lane >> 3, col = lane & 7;
-    const T* from = reinterpret_cast<const T*>(base) + l.b * sb + (l.d - lane * V) + col * 4 * V + (int64_t)(t0 + row) * st;
+    const T* from = reinterpret_cast<const T*>(base) + b * sb + d + (int64_t)(t0 + row) * st;
     unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, which, row) - lane + 4 * col);
 #pragma unroll
     for (int i = 0; i < CHUNK / 4; i++) {
@@ -444,13 +451,15 @@ template <typename T, int V> struct Inputs<T, V, true> {
       advance(from, 4 * st);
     }
   }
-  __device__ __forceinline__ void fetch(const Args& p, const Lane& l, int stage, int t0, int n) {
+  __device__ __forceinline__ void fetch(const Args& p, const Lane& l, int stage, int t0, bool there) {
     if (rows) {
       __syncwarp();             // every lane has read what this stage held
-      copy_rows(stage, 0, p.gate, p.gate_t, p.gate_b, l, t0, n);
-      copy_rows(stage, 1, p.x, p.x_t, p.x_b, l, t0, n);
-      if (with_dh) copy_rows(stage, 2, p.dh, p.dh_t, p.dh_b, l, t0, n);
+      const int m = there ? len - t0 : 0;
+      copy_rows(stage, 0, p.gate, p.gate_t, p.gate_b, t0, m);
+      copy_rows(stage, 1, p.x, p.x_t, p.x_b, t0, m);
+      if (with_dh) copy_rows(stage, 2, p.dh, p.dh_t, p.dh_b, t0, m);
     } else {
+      const int n = there ? steps_of(l, t0) : 0;
       const Line<T> g(p.gate, p.gate_t, p.gate_b, l, t0), x(p.x, p.x_t, p.x_b, l, t0), d(p.dh, p.dh_t, p.dh_b, l, t0);
       copy(stage, 0, g, n);
       copy(stage, 1, x, n);
@@ -556,13 +565,13 @@ __global__ void __launch_bounds__(32 * WARPS, GRAD_BLOCKS)
   const auto saved_at = [&](int t0) {
     return load_state<V>(t0 >= begin && steps_of(l, t0) > 0 ? p.saved + (int64_t)(t0 / CHUNK) * channels : nullptr, l);
   };
-  if constexpr (STAGED) in.fetch(p, l, 0, first, steps_of(l, first));
+  if constexpr (STAGED) in.fetch(p, l, 0, first, true);
   P h = saved_at(first), h_next = h;
   bool ahead = reset_ahead(p, l, first);
   for (int t0 = first; t0 >= begin; t0 -= CHUNK, h = h_next) {
     const int n = steps_of(l, t0), left = steps - t0, next = t0 - CHUNK;
     const unsigned cut = resets_of(p, l, t0, ahead);
-    if constexpr (STAGED) in.fetch(p, l, stage ^ 1, next, next >= begin ? steps_of(l, next) : 0);
+    if constexpr (STAGED) in.fetch(p, l, stage ^ 1, next, next >= begin);
     h_next = saved_at(next);
     if (next >= begin) ahead = reset_ahead(p, l, next);
     if constexpr (STAGED) in.wait();

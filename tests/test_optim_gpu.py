@@ -389,6 +389,25 @@ def test_captured_step_counts(cuda, bits):
         assert torch.equal(opts[a].grad_norm, opts[b].grad_norm)
 
 
+def test_two_optimisers_at_once(cuda):
+    """Actor's and critic's steps on two streams: the bits of one after the other."""
+    opt_mod = pkg_module("optim")
+    sets = [make(cuda, torch.float32, s) for s in (14, 14, 15, 15)]
+    opts = [opt_mod.AdamW(ps, lr=1e-2, state_bits=8, max_grad_norm=1.0) for ps in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for st, o in zip(streams, (opts[0], opts[2])):
+            with torch.cuda.stream(st):
+                o.step()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        opts[1].step()
+        opts[3].step()
+    for a, b in ((0, 1), (2, 3)):
+        assert all(torch.equal(p, q) for p, q in zip(sets[a], sets[b]))
+
+
 def test_writes_are_seen_by_autograd(cuda):
     """A step changes its parameters' versions, as torch's optimisers do: a backward pass over values saved
     before it refuses."""

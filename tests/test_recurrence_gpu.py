@@ -9,6 +9,8 @@ coefficients first, which rounds once more per step.  C = 96 covers all of it.  
 recurrence is bounded the same way, with the states' bound on top; the product that makes dgate
 adds 8 C.  A value of type T then is off by its rounding, finfo(T).eps / 2 of itself.
 """
+import ctypes
+
 import pytest
 import torch
 
@@ -218,6 +220,72 @@ def test_partial_gradients(cuda):
     want, tol = reference(e, True, dh, zero_n)
     total = want["dgate"].sum((0, 1))
     assert bool(((got.double() - total).abs() <= tol["dgate"].sum((0, 1)) + 280 * H * want["dgate"].abs().sum((0, 1))).all())
+
+
+# several sequences to a warp, with widths that fit 16-byte copies (8, 16, 24), that do not (5, 14), and more
+# sequences than a ballot has halves for (1, 2)
+@pytest.mark.parametrize("batch,dim", [(75, 1), (70, 2), (40, 5), (33, 8), (21, 14), (70, 16), (9, 24)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gated", [True, False])
+def test_sequences_that_share_a_warp(cuda, batch, dim, dtype, gated):
+    for steps, batch_first in ((50, False), (333, True)):
+        d, dh, dhn = make(cuda, steps, batch, dim, dtype, gated, dim, resets=True, padded=True, batch_first=batch_first)
+        want, tol = reference(d, gated, dh, dhn)
+        check(run(d, gated, dh, dhn), want, tol)
+
+
+def call(entry, d, gated, scratch, **buffers):
+    """A C entry on time-major fp32 tensors, with the scratch given (None: time is not cut)."""
+    _lib = pkg_module("_lib")
+    rec = pkg_module("recurrence")
+    b = {**dict.fromkeys(("h", "hn", "saved", "dh", "dhn", "dgate", "dx", "dh0")), **buffers}
+    a = rec._args(d["gate"], d["x"], d["h0"], d["reset"], d["lengths"], int(gated), b["h"], b["hn"], b["saved"],
+                  (scratch, 0 if scratch is None else scratch.numel()), b["dh"], b["dhn"], b["dgate"], b["dx"], b["dh0"])
+    _lib.check(getattr(_lib.load(), entry)(ctypes.byref(a), _lib.stream_of(d["x"])), entry)
+
+
+@pytest.mark.parametrize("steps,batch,dim", [(5000, 3, 7), (600_000, 1, 1)])
+def test_cut_and_uncut_time(cuda, steps, batch, dim):
+    """With scratch time is cut into segments (600,000 steps: more than the 1,024 whose states are joined at a
+    time), without it is not: both are within the bound of the recurrence, so within twice the bound of each
+    other.  The bound of |a| <= 0.9: errors of C half steps a step add up to at most C H (|a h| + |x|) / 0.1."""
+    _lib = pkg_module("_lib")
+    g = torch.Generator(device=cuda).manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, device=cuda, generator=g)
+    d = dict(gate=rnd(steps, batch, dim).clamp(-0.9, 0.9), x=rnd(steps, batch, dim), h0=rnd(batch, dim),
+             reset=torch.rand(steps, batch, device=cuda, generator=g) < 0.01, lengths=None)
+    dh, dhn = rnd(steps, batch, dim), rnd(batch, dim)
+    n = _lib.load().f16_scan_scratch_floats(steps, batch, dim)
+    assert n > 0
+    out = []
+    for scratch in (None, torch.empty(n, device=cuda), torch.empty(n - 1, device=cuda)):
+        saved = torch.empty(_lib.load().f16_scan_saved_floats(steps, batch, dim), device=cuda)
+        o = dict(h=torch.empty_like(d["x"]), hn=torch.empty(batch, dim, device=cuda))
+        call("f16_scan_fwd", d, False, scratch, saved=saved, **o)
+        q = dict(dgate=torch.empty_like(dh), dx=torch.empty_like(dh), dh0=torch.empty(batch, dim, device=cuda))
+        call("f16_scan_bwd", d, False, scratch, saved=saved, dh=dh, dhn=dhn, **q)
+        out.append({**o, **q})
+    top = {"h": 1.0, "hn": 1.0, "dx": 1.0, "dh0": 1.0, "dgate": float(out[0]["h"].abs().max())}
+    for name, v in out[0].items():
+        bound = 4 * C * H * 10 * (float(v.abs().max()) + top[name] * float(d["x"].abs().max()))
+        assert float((v - out[1][name]).abs().max()) <= bound, name
+        assert torch.equal(v, out[2][name])                # too little scratch: as without
+
+
+def test_two_scans_at_once(cuda):
+    """On two streams, each with scratch of its own: the bits of one after the other."""
+    cases = [make(cuda, 3000, 2, 40, torch.bfloat16, True, s, resets=True) for s in (1, 2)]
+    want = [run(d, True, dh, dhn) for d, dh, dhn in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for st, (d, dh, dhn) in zip(streams, cases):
+            with torch.cuda.stream(st):
+                got.append(run(d, True, dh, dhn))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(a[n], b[n]) for n in b)
 
 
 def test_no_gradient_saves_no_states(cuda):

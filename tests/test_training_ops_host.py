@@ -34,6 +34,7 @@ def test_layer_norm_entries_refuse(buf):
     assert bwd(dy=None) == ARG and bwd(m=None) == ARG and bwd(rows=0) == ARG and bwd(dt=9) == ARG
     assert bwd(s=None) == ARG and bwd(n=15) == ARG             # no room for one block's sums
     assert bwd(dx=None, dw=None) == 0                          # nothing wanted
+    assert fwd(cols=2 ** 29 + 1, ldy=2 ** 30) == TOO_LARGE
     assert lib.f16_layer_norm_scratch_floats(0, 8) == 0
     assert lib.f16_layer_norm_scratch_floats(3, 8) == 2 * 8 * 3
 
@@ -58,9 +59,14 @@ def test_scan_entries_refuse(buf):
         assert call(fn, steps=2 ** 31) == TOO_LARGE
         assert call(fn, x=p.value + 2) == ALIGN
         assert call(fn, reset=p.value + 1, reset_bytes=4) == ALIGN
+        assert call(fn, scratch=p.value + 4) == ALIGN
+        assert call(fn, batch=2 ** 40, dim=2 ** 40) == TOO_LARGE
     assert call(lib.f16_scan_fwd, h=None) == ARG
     assert call(lib.f16_scan_bwd, saved=None) == ARG and call(lib.f16_scan_bwd, dh=None) == ARG
     assert lib.f16_scan_saved_floats(17, 2, 3) == 2 * 6 and lib.f16_scan_saved_floats(0, 2, 3) == 0
+    # one chunk, or channels enough for every SM: time is not cut; else three floats a segment and channel
+    assert lib.f16_scan_scratch_floats(16, 1, 8) == 0 and lib.f16_scan_scratch_floats(64, 16384, 128) == 0
+    assert lib.f16_scan_scratch_floats(32, 1, 8) == 3 * 2 * 8 and lib.f16_scan_scratch_floats(-1, 1, 8) == 0
     step = lambda gate=p, state=p, dt=2, sb=4, hb=4, batch=2, rb=0, reset=None: \
         lib.f16_scan_step(gate, 4, p, 4, batch, 4, dt, 1, reset, rb, 1, state, sb, p, hb, None)
     assert step(gate=None) == ARG and step(state=None) == ARG and step(batch=0) == ARG and step(dt=5) == ARG
@@ -134,6 +140,7 @@ def test_constants_match_the_header():
                            torch.float32: define("F16_DTYPE_FP32")}
     assert pkg_module("optim").BLOCK == define("F16_ADAMW_BLOCK")
     assert pkg_module("recurrence").CHUNK == define("F16_SCAN_CHUNK")
+    assert pkg_module("layernorm").MAX_DIM == 2 ** 29
 
 
 def test_wrappers_refuse_cpu_tensors():
