@@ -34,7 +34,8 @@ constexpr int CHUNK = F16_SCAN_CHUNK;     // steps in registers at a time, betwe
 constexpr int WARPS = 4;                  // of a block, each with channels (and a segment) of its own
 // Blocks on an SM: 96, 128 and 80 registers a thread.
 constexpr int WALK_BLOCKS = 5, GRAD_BLOCKS = 4, FOLD_BLOCKS = 6;
-constexpr int MAX_SEGMENT = F16_SCAN_SEGMENT;      // steps whose coefficients' product is formed
+constexpr int MAX_SEGMENT = F16_SCAN_SEGMENT;      // most steps of a segment
+constexpr int64_t MAX_STEPS = 0x7fffffff - 2 * CHUNK;     // time indexes are 32-bit
 // Time is cut where the channels give fewer than ENOUGH_PER_SM warps an SM, into so many segments that there
 // are WARPS_PER_SM, but no more than MAX_CUTS (k_scan_starts takes so many at once) while they are not too long.
 constexpr int ENOUGH_PER_SM = 12, WARPS_PER_SM = 64, MAX_CUTS = 1024;
@@ -475,19 +476,19 @@ template <typename T, int V> struct Inputs<T, V, true> {
 };
 template <typename T, int V> struct Inputs<T, V, false> {
   typedef int Buffer;
-  Vec<T, V> in[STAGES][3][CHUNK];
+  Vec<T, V> in[3][CHUNK];
   bool with_dh;
   __device__ __forceinline__ Inputs(Buffer&, const Args& p, const Lane&) : with_dh(p.dh) {}
-  __device__ __forceinline__ Vec<T, V> gate(int, int i) const { return in[0][0][i]; }
-  __device__ __forceinline__ Vec<T, V> x(int, int i) const { return in[0][1][i]; }
+  __device__ __forceinline__ Vec<T, V> gate(int, int i) const { return in[0][i]; }
+  __device__ __forceinline__ Vec<T, V> x(int, int i) const { return in[1][i]; }
   __device__ __forceinline__ typename Lanes<V>::type dh(int, int i) const {
-    return with_dh ? widen(in[0][2][i]) : all_of<typename Lanes<V>::type>(0.0f);
+    return with_dh ? widen(in[2][i]) : all_of<typename Lanes<V>::type>(0.0f);
   }
   __device__ __forceinline__ void load(const Args& p, const Lane& l, int t0, int n) {
     const bool all = __all_sync(~0u, n == CHUNK);
-    load_chunk<T, V>(in[0][0], Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
-    load_chunk<T, V>(in[0][1], Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
-    if (with_dh) load_chunk<T, V>(in[0][2], Line<T>(p.dh, p.dh_t, p.dh_b, l, t0), n, all);
+    load_chunk<T, V>(in[0], Line<T>(p.gate, p.gate_t, p.gate_b, l, t0), n, all);
+    load_chunk<T, V>(in[1], Line<T>(p.x, p.x_t, p.x_b, l, t0), n, all);
+    if (with_dh) load_chunk<T, V>(in[2], Line<T>(p.dh, p.dh_t, p.dh_b, l, t0), n, all);
   }
 };
 
@@ -699,7 +700,7 @@ inline int check(const Args* p, bool grad) {
     return F16_ERR_ARG;
   if (p->dtype != F16_DTYPE_BF16 && p->dtype != F16_DTYPE_FP16 && p->dtype != F16_DTYPE_FP32) return F16_ERR_ARG;
   if (grad ? !p->saved || (!p->dh && !p->dhn) : !p->h) return F16_ERR_ARG;
-  if (p->steps > 0x7fffffff - 2 * CHUNK || p->batch > INT64_MAX / 16 / p->dim) return F16_ERR_TOO_LARGE;
+  if (p->steps > MAX_STEPS || p->batch > INT64_MAX / 16 / p->dim) return F16_ERR_TOO_LARGE;
   const int size = p->dtype == F16_DTYPE_FP32 ? 4 : 2;
   if (!aligned(p->gate, size) || !aligned(p->x, size) || !aligned(p->h, size) || !aligned(p->dh, size) ||
       !aligned(p->dgate, size) || !aligned(p->dx, size) || (p->reset && p->reset_bytes == 4 && !aligned(p->reset, 4)) ||
@@ -745,7 +746,7 @@ extern "C" int64_t f16_scan_saved_floats(int64_t steps, int64_t batch, int64_t d
 }
 
 extern "C" int64_t f16_scan_scratch_floats(int64_t steps, int64_t batch, int64_t dim) {
-  if (steps <= 0 || batch <= 0 || dim <= 0 || batch > INT64_MAX / 16 / dim) return 0;
+  if (steps <= 0 || batch <= 0 || dim <= 0 || batch > INT64_MAX / 16 / dim || steps > scan::MAX_STEPS) return 0;
   const int64_t one = scan::scratch_for(scan::shape_for(batch * dim, steps, 1), batch * dim),
                 two = scan::scratch_for(scan::shape_for(batch * dim, steps, 2), batch * dim);
   return one > two ? one : two;

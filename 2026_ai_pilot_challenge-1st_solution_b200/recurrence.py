@@ -143,7 +143,7 @@ def gated_scan(gate, x, h0=None, reset=None, lengths=None):
 
 def linear_scan(a, x, h0=None, reset=None, lengths=None):
     """(h, hn) of h_t = a_t h_{t-1} + x_t; arguments as in ``gated_scan``.  Meant for coefficients of
-    size up to 1; the product of 512 successive ones has to stay in fp32's range."""
+    size up to 1; the product of 8,192 successive ones has to stay in fp32's range."""
     return _scan(a, x, h0, reset, lengths, False, "linear_scan")
 
 

@@ -552,7 +552,8 @@ int64_t f16_layer_norm_scratch_floats(int64_t rows, int cols);
  * dh and dhn (one of them may be NULL: zero) and writes dgate, dx and dh0, each NULL where not
  * wanted.  scratch: f16_scan_scratch_floats values, 8-byte aligned (none of them are kept); with less or
  * NULL, time is not cut into segments, which is slow for few channels and many steps.  Coefficients
- * above 1 in size: the product of any F16_SCAN_SEGMENT successive ones has to stay in fp32's range. */
+ * above 1 in size: the product of any 16 F16_SCAN_SEGMENT successive ones has to stay in fp32's range.
+ * steps below 2^31 - 32. */
 #define F16_SCAN_CHUNK 16
 #define F16_SCAN_SEGMENT 512
 typedef struct {

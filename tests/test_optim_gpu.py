@@ -500,3 +500,20 @@ def test_update_of_the_trainer(cuda):
         assert abs(a - b) <= 1e-4 * abs(a)
     with pytest.raises(ValueError):
         tr.make_optimizer(base.actor_parameters(), 1e-3, tr.PPOConfig(optimizer="sgd"))
+
+
+def test_trainer_iteration(cuda):
+    """PPOTrainer with 8-bit AdamW: rollout, update, the policy kernel's weights refreshed; finite throughout."""
+    rl_env, tr, optim = pkg_module("rl_env"), pkg_module("trainer"), pkg_module("optim")
+    env = rl_env.GpuDogfightVecEnv(256, substeps=6, seed=5)
+    torch.manual_seed(5)
+    cfg = tr.PPOConfig(rollout_steps=4, hidden=(128, 128), activation="tanh", update_epochs=2, num_minibatches=2,
+                       target_kl=None, optimizer="adamw", weight_decay=1e-3, state_bits=8)
+    t = tr.PPOTrainer(env, cfg, opponents=[tr.Opponent(tr.MLPActorCritic(hidden=(128, 128)).to(cuda))])
+    assert isinstance(t.actor_opt, optim.AdamW) and isinstance(t.critic_opt, optim.AdamW)
+    before = [p.detach().clone() for p in t.model.parameters()]
+    res, _ = t.iteration()
+    assert res["optimizer_steps"] == 4 and float(res["actor_grad_norm"]) > 0
+    assert bool((t.actor_opt.state_buffers()[0]["step"] == 4).all())
+    for p, q in zip(t.model.parameters(), before):
+        assert bool(p.isfinite().all()) and not torch.equal(p, q)
