@@ -12,6 +12,10 @@
 // backward pass so do the columns' partial sums of dw and db, which leave the block once, to be
 // added up by k_ln_wgrad in a fixed order (no atomics: the same inputs give the same gradients).
 // Sums, statistics and partial sums are fp32; values are rounded once, when stored.
+//
+// Sums of products are made of products rounded by themselves (pairs of values are multiplied by adding a
+// zero that the assembler does not know to be one; it would fuse the product with the sum after it): what
+// cancels in the formulas then cancels in fp32 -- a row of one value has no gradient, of two values hardly one.
 #include "typed.cuh"
 
 namespace f16 {
@@ -30,6 +34,7 @@ struct Weights {
   const void* w;
   const void* b;
   int dtype;
+  float minus_zero;
 };
 
 // V of them from i on, a multiple of V: 16 bytes a load where the weights are aligned so.
@@ -313,9 +318,10 @@ __global__ void __maxnreg__(80)
         v[i] = two(at.there >> (2 * i / V) & 1 ? f.x : 0.0f, at.there >> ((2 * i + 1) / V) & 1 ? f.y : 0.0f);
       }
     }
+    const Two zero = two(wb.minus_zero);
     s[0] = s[1] = two(0.0f);
 #pragma unroll
-    for (int i = 0; i < E / 2; i++) s[i & 1] = fma2(v[i], v[i], s[i & 1]);
+    for (int i = 0; i < E / 2; i++) s[i & 1] = s[i & 1] + fma2(v[i], v[i], zero);
     total[0] = sum_of(s);
     row_sums<LANES, 1>(total, at.lanes, red, half);
     const float r = rsqrtf(total[0] * inv + eps);
@@ -371,7 +377,7 @@ __global__ void __maxnreg__(128)
     ring.take(here);
     put();
     const Part<T, V, E>&cx = here[0], &cg = here[1];
-    const Two minus = two(-nmu), scale = two(nr);
+    const Two minus = two(-nmu), scale = two(nr), zero = two(wb.minus_zero);
     const float r = nr;
     nmu = row + step < rows ? mean[row + step] : 0.0f;
     nr = row + step < rows ? rstd[row + step] : 0.0f;
@@ -379,9 +385,9 @@ __global__ void __maxnreg__(128)
     if (row < rows) {
 #pragma unroll
       for (int i = 0; i < E / 2; i++) {
-        const Two d = cg.pair(i), xh = (cx.pair(i) + minus) * scale, g = d * w[i];
+        const Two d = cg.pair(i), xh = (cx.pair(i) + minus) * scale, g = fma2(d, w[i], zero);
         s1 = s1 + g;
-        s2 = fma2(g, xh, s2);
+        s2 = s2 + fma2(g, xh, zero);
         aw[i] = fma2(d, xh, aw[i]);
         ab[i] = ab[i] + d;
       }
@@ -391,13 +397,12 @@ __global__ void __maxnreg__(128)
     float total[2] = {f1.x + f1.y, f2.x + f2.y};
     row_sums<LANES, 2>(total, at.lanes, red, half);
     if (row < rows) {
-      // dx = r g - r m1 - xh r m2
       const Two m1 = two(-total[0] * inv), m2 = two(-total[1] * inv), rr = two(r);
       Part<T, V, E> out;
 #pragma unroll
       for (int i = 0; i < E / 2; i++) {
-        const Two xh = (cx.pair(i) + minus) * scale, g = cg.pair(i) * w[i];
-        out.set(i, fma2(xh, m2, g + m1) * rr);
+        const Two xh = (cx.pair(i) + minus) * scale, g = fma2(cg.pair(i), w[i], zero);
+        out.set(i, ((g + m1) + fma2(xh, m2, zero)) * rr);
       }
       out.store(to, at.apart, at.there, at.full);
     }
@@ -745,7 +750,7 @@ extern "C" int f16_layer_norm_fwd(const void* x, int64_t rows, int cols, int64_t
   if (!aligned(x, ln::size_of(dtype)) || !aligned(y, ln::size_of(dtype)) || !aligned(weight, ln::size_of(wdtype)) ||
       !aligned(bias, ln::size_of(wdtype)))
     return F16_ERR_ALIGN;
-  const ln::Weights wb = {weight, bias, wdtype};
+  const ln::Weights wb = {weight, bias, wdtype, -0.0f};
   const cudaStream_t st = cu_stream(stream);
   if (dtype == F16_DTYPE_FP32)
     return ln::forward((const float*)x, rows, cols, ldx, wb, (float)eps, (float*)y, ldy, mean, rstd, st);
@@ -775,7 +780,7 @@ extern "C" int f16_layer_norm_bwd(const void* dy, int64_t ldg, const void* x, in
   const int size = ln::size_of(dtype);
   if (!aligned(dy, size) || !aligned(x, size) || !aligned(dx, size) || !aligned(weight, ln::size_of(wdtype)))
     return F16_ERR_ALIGN;
-  const ln::Weights wb = {weight, nullptr, wdtype};
+  const ln::Weights wb = {weight, nullptr, wdtype, -0.0f};
   float* part = sums ? scratch : nullptr;
   const cudaStream_t st = cu_stream(stream);
   if (dtype == F16_DTYPE_FP32)

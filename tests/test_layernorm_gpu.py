@@ -162,6 +162,28 @@ def test_special_values(cuda):
     check(ln.layer_norm(far, eps=100.0), want[0], tol[0], "y")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_cancels(cuda, dtype):
+    """A row of one value has no gradient, exactly; of rows of two (xh = +-1 but for eps) the gradient is what
+    remains of much larger terms. In half steps H of fp32, with d = x - mu and q = |mu| / |d|: mu is rounded
+    once, d is off by q + 1 of itself; in the variance the mean's part cancels to second order, which leaves
+    2 + 1 + 1 and 1 for eps, so r is off by 2.5 and its own 4, at most 7, and xh by q + 9. g is off by 1, m1 by
+    2, m2 by q + 12, xh m2 by 2 q + 22, the two sums add 2 of at most 2 terms' size each, and r with its product
+    8 more: below 2 q + 40 of r max|g|, and twice the q for its second order."""
+    x, w, b, dy = make(cuda, 300, 1, dtype, torch.float32, 1)
+    y, dx, dw, db = run(x, w, b, dy)
+    assert bool((dx == 0).all()) and bool((dw == 0).all()) and torch.equal(y, b.to(dtype).expand(300, 1))
+    x, w, b, dy = make(cuda, 300, 2, dtype, torch.float32, 2)
+    want, _ = reference(x, w, b, dy, 1e-5)
+    got = run(x, w, b, dy)[1]
+    r = 1 / torch.sqrt(x.double().var(-1, unbiased=False, keepdim=True) + 1e-5)
+    mu = x.double().mean(-1, keepdim=True)
+    q = mu.abs() / (x.double() - mu).abs().amax(-1, keepdim=True).clamp_min(1e-300)
+    size = r * (dy.double() * w.double()).abs().amax(-1, keepdim=True)
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((got.double() - want[1]).abs() <= (4 * q + 40) * H * size + half * want[1].abs()).all())
+
+
 def test_empty(cuda):
     ln = pkg_module("layernorm")
     x = torch.zeros(0, 5, device=cuda, requires_grad=True)
