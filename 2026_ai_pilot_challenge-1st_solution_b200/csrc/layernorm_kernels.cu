@@ -16,6 +16,10 @@
 // Sums of products are made of products rounded by themselves (pairs of values are multiplied by adding a
 // zero that the assembler does not know to be one; it would fuse the product with the sum after it): what
 // cancels in the formulas then cancels in fp32 -- a row of one value has no gradient, of two values hardly one.
+//
+// Measured on a B200 whose copy makes 6.55 TB/s, with a cold L2 (forward / backward / k_ln_wgrad, us, and the
+// share of that rate): 524,288 x 512 fp32 353 / 512 / 4 (93%, 96%); 16,384 x 4,096 bf16 47 / 80 / 4 (88%, 77%);
+// 100,003 x 215 fp16, in loads of 2 bytes, 28 / 42 / 3 (48%, 47%); 128 x 184 fp32, forward alone, 2.8.
 #include "typed.cuh"
 
 namespace f16 {
@@ -158,7 +162,8 @@ struct Part {
 };
 
 // The thread's parts of its next rows, N tensors' of each: on their way into shared memory two rows ahead
-// (one row a block in flight leaves HBM idle half of the time), or, where a load is narrower than the 4 bytes
+// (one row a block in flight leaves HBM idle half of the time; 16,384 x 4,096 bf16, forward + backward: 2 / 3 / 4
+// slots 52 + 81, 44 + 79, 45 + 79 us, and 80 + 106 from registers), or, where a load is narrower than the 4 bytes
 // that can be copied so, one row ahead in registers.  A thread reads what it copied itself, so no barrier.
 constexpr int SLOTS = 3;
 template <typename T, int V, int E, int N>
@@ -464,7 +469,8 @@ __device__ __forceinline__ float wide_sum(float v, float (*red)[1][32], int& hal
 }
 
 // Rows too wide for a block's registers: a block a row, V values a load, read again for each of the passes
-// (the second and third hit L1 and L2).
+// (the second and third hit L1 and L2).  4,096 x 16,384 bf16, forward and backward with the sums over rows: 285 us,
+// where one read of everything would take 102.
 template <typename T, int V>
 __global__ void __launch_bounds__(WIDE)
     k_ln_fwd_wide(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps,
@@ -633,7 +639,9 @@ inline int64_t grid_rows(int64_t rows, const Plan& p, int warps_per_sm) {
   return need < most ? need : most;
 }
 
-constexpr int FWD_WARPS = 24, BWD_WARPS = 16;    // persistent warps per SM
+// Persistent warps per SM, which the registers allow (80 and 128 a thread).  Forward with 16 / 24 / 32 of them:
+// 16,384 x 4,096 bf16 49 / 44 / 54 us, 100,003 x 215 fp16 37 / 31 / 41.
+constexpr int FWD_WARPS = 24, BWD_WARPS = 16;
 
 // Dynamic shared memory above 48 KB has to be asked for (on every device; it costs the host under a microsecond).
 template <typename K>

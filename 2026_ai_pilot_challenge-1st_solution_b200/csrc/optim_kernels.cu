@@ -21,6 +21,11 @@
 //
 // 16-bit parameters may have fp32 master copies; a master counts while it rounds to its parameter,
 // else the parameter was set from outside and is taken instead.
+//
+// Measured on a B200 whose copy makes 6.55 TB/s (norm + update, us): 252 million fp32 parameters with 8-bit moments
+// 165 + 811 (93%, 76% of that rate), 300 tensors with 22 million bf16 parameters, fp32 moments and masters 14 + 123,
+// 1.3 million fp32 parameters 2.5 + 8.2.  The 8-bit update is bound by the instructions of its roundings (integer
+// pipe 60%, 2.7 of 4 issue slots), not by HBM; pairs of values in one instruction brought it from 956 to 847.
 #include <cuda_fp8.h>
 #include "typed.cuh"
 
@@ -28,7 +33,8 @@ namespace f16 {
 namespace opt {
 
 constexpr int THREADS = 256;
-// Resident update blocks, each walking over its share: 64 registers a thread (80 and three blocks: +4% with 8-bit moments).
+// Resident update blocks, each walking over its share: 64 registers a thread (80 and three blocks: +4% with 8-bit moments,
+// +7% with the next block's values copied to shared memory ahead).
 constexpr int BLOCKS_PER_SM = 4;
 constexpr int NORM_BLOCKS_PER_SM = 4;
 constexpr int QBLOCK = F16_ADAMW_BLOCK;       // values of one scale: a warp's, 8 each
