@@ -3,6 +3,9 @@
 Modules mirror the reference's names for the path:
   gpu_env     GpuDogfight                         (cuda_fdm/gpu_env.py)
   ic          IC geodesy, sampling, GPU seeding   (cuda_fdm/ic.py, rl_env.py:57-174)
+  layernorm   layer_norm, LayerNorm               (no counterpart)
+  recurrence  gated / linear recurrence, its step (no counterpart)
+  optim       AdamW                               (torch.optim.Adam, ppo_gpu.py:1300)
   _lib        ctypes binding of libf16env.so (include/f16env.h)
   build       in-tree nvcc build of libf16env.so for sm_100a
 
