@@ -13,12 +13,12 @@
 // added up by k_ln_wgrad in a fixed order (no atomics: the same inputs give the same gradients).
 // Sums, statistics and partial sums are fp32; values are rounded once, when stored.
 //
-// Sums of products are made of products rounded by themselves (pairs of values are multiplied by adding a
+// Rows of a warp or less: sums of products are made of products rounded by themselves (pairs of values are multiplied by adding a
 // zero that the assembler does not know to be one; it would fuse the product with the sum after it): what
 // cancels in the formulas then cancels in fp32 -- a row of one value has no gradient, of two values hardly one.
 //
 // Measured on a B200 whose copy makes 6.55 TB/s, with a cold L2 (forward / backward / k_ln_wgrad, us, and the
-// share of that rate): 524,288 x 512 fp32 353 / 512 / 4 (93%, 96%); 16,384 x 4,096 bf16 47 / 80 / 4 (88%, 77%);
+// share of that rate): 524,288 x 512 fp32 353 / 512 / 4 (93%, 96%); 16,384 x 4,096 bf16 44 / 79 / 4 (93%, 78%);
 // 100,003 x 215 fp16, in loads of 2 bytes, 28 / 42 / 3 (48%, 47%); 128 x 184 fp32, forward alone, 2.8.
 #include "typed.cuh"
 
@@ -272,6 +272,14 @@ __device__ __forceinline__ float sum_of(const Two (&s)[2]) {
   return f.x + f.y;
 }
 
+// s + a b with the product rounded by itself; where a row takes a block nothing is left to cancel, and the fused
+// operation saves a tenth of the forward pass (16,384 x 4,096 bf16 44 us for 47, backward 79 for 80).
+template <int LANES>
+__device__ __forceinline__ Two plus_product(Two s, Two a, Two b, Two zero) {
+  if constexpr (LANES == ROW_BLOCK) return fma2(a, b, s);
+  else return s + fma2(a, b, zero);
+}
+
 template <typename T, int V, int E, int LANES>
 __global__ void __maxnreg__(80)
     k_ln_fwd(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps, T* __restrict__ y,
@@ -326,7 +334,7 @@ __global__ void __maxnreg__(80)
     const Two zero = two(wb.minus_zero);
     s[0] = s[1] = two(0.0f);
 #pragma unroll
-    for (int i = 0; i < E / 2; i++) s[i & 1] = s[i & 1] + fma2(v[i], v[i], zero);
+    for (int i = 0; i < E / 2; i++) s[i & 1] = plus_product<LANES>(s[i & 1], v[i], v[i], zero);
     total[0] = sum_of(s);
     row_sums<LANES, 1>(total, at.lanes, red, half);
     const float r = rsqrtf(total[0] * inv + eps);
@@ -390,9 +398,9 @@ __global__ void __maxnreg__(128)
     if (row < rows) {
 #pragma unroll
       for (int i = 0; i < E / 2; i++) {
-        const Two d = cg.pair(i), xh = (cx.pair(i) + minus) * scale, g = fma2(d, w[i], zero);
+        const Two d = cg.pair(i), xh = (cx.pair(i) + minus) * scale, g = LANES == ROW_BLOCK ? d * w[i] : fma2(d, w[i], zero);
         s1 = s1 + g;
-        s2 = s2 + fma2(g, xh, zero);
+        s2 = plus_product<LANES>(s2, g, xh, zero);
         aw[i] = fma2(d, xh, aw[i]);
         ab[i] = ab[i] + d;
       }
@@ -406,8 +414,8 @@ __global__ void __maxnreg__(128)
       Part<T, V, E> out;
 #pragma unroll
       for (int i = 0; i < E / 2; i++) {
-        const Two xh = (cx.pair(i) + minus) * scale, g = fma2(cg.pair(i), w[i], zero);
-        out.set(i, ((g + m1) + fma2(xh, m2, zero)) * rr);
+        const Two xh = (cx.pair(i) + minus) * scale, g = LANES == ROW_BLOCK ? cg.pair(i) * w[i] : fma2(cg.pair(i), w[i], zero);
+        out.set(i, plus_product<LANES>(g + m1, xh, m2, zero) * rr);
       }
       out.store(to, at.apart, at.there, at.full);
     }
