@@ -26,7 +26,7 @@ namespace f16 {
 namespace ln {
 
 constexpr int BLOCK = 256;          // threads of a block whose rows take a warp or less
-constexpr int MAX_LANES = 512;      // threads of a row: 128 registers each
+constexpr int MAX_LANES = 512, FWD_LANES = 768;      // threads of a row, at most: see most_of
 // Most values of a row in one thread.  16-byte loads take so many; with narrower ones a thread takes 8, of rows
 // up to 16 values 4 (500,000 x 33 fp16, forward + backward: 8 a thread 100 us, 4 142 us, 2 188 us;
 // 300,000 x 15 bf16: 30, 25 and 36 us), and 16 again where 8 do not suffice.
@@ -60,18 +60,21 @@ __device__ __forceinline__ void load_weights_of(float (&w)[V], const W* p) {
 #pragma unroll
   for (int k = 0; k < V; k++) w[k] = to_f32(p[k]);
 }
-template <int V>
-__device__ __forceinline__ void load_weights(float (&w)[V], const void* p, int dtype, int64_t i, float none) {
+template <int V, typename W>
+__device__ __forceinline__ void load_weights(float (&w)[V], const void* p, int64_t i, float none) {
   if (!p) {
 #pragma unroll
     for (int k = 0; k < V; k++) w[k] = none;
-  } else if (dtype == F16_DTYPE_FP32) {
-    load_weights_of<V>(w, reinterpret_cast<const float*>(p) + i);
-  } else if (dtype == F16_DTYPE_BF16) {
-    load_weights_of<V>(w, reinterpret_cast<const __nv_bfloat16*>(p) + i);
   } else {
-    load_weights_of<V>(w, reinterpret_cast<const __half*>(p) + i);
+    load_weights_of<V>(w, reinterpret_cast<const W*>(p) + i);
   }
+}
+// f(a value of the weights' type).
+template <typename F>
+__device__ __forceinline__ void of_weights(int dtype, F f) {
+  if (dtype == F16_DTYPE_FP32) f(0.0f);
+  else if (dtype == F16_DTYPE_BF16) f(__nv_bfloat16());
+  else f(__half());
 }
 __device__ __forceinline__ void store_from_f32(void* p, int dtype, int64_t i, float v) {
   if (dtype == F16_DTYPE_FP32) reinterpret_cast<float*>(p)[i] = v;
@@ -476,25 +479,37 @@ __device__ __forceinline__ float wide_sum(float v, float (*red)[1][32], int& hal
   return t[0];
 }
 
+// The block's next row into L2, a line of 128 bytes a thread, while the present one's sums are made: forward with
+// narrow loads only (13,000 x 9,001 fp32 245 -> 204 us; with 16-byte loads, and backward with any, it lost).
+template <typename T>
+__device__ __forceinline__ void fetch_ahead(const T* row, int cols) {
+  constexpr int LINE = 128 / (int)sizeof(T);
+  for (int c = threadIdx.x * LINE; c < cols; c += WIDE * LINE) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
+}
+
 // Rows too wide for a block's registers: a block a row, V values a load, read again for each of the passes
-// (the second and third hit L1 and L2).  4,096 x 16,384 bf16, forward and backward with the sums over rows: 285 us,
-// where one read of everything would take 102.
+// (the second and third hit L1 and L2), several loads under way a thread: 4,096 x 16,384 bf16 90 us forward, 92 + 52
+// + 10 backward with the sums over rows, where one read of everything would take 41 and 61.
 template <typename T, int V>
-__global__ void __launch_bounds__(WIDE)
+__global__ void __launch_bounds__(WIDE, WIDE_PER_SM)
     k_ln_fwd_wide(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps,
                   T* __restrict__ y, int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd) {
   __shared__ float red[2][1][32];
+  constexpr int UNROLL = V == 1 ? 8 : 2;
   int half = 0;
   const float inv = 1.0f / (float)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
     float s = 0.0f, q = 0.0f;
+#pragma unroll UNROLL
     for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
       const Vec<T, V> v = load_vec<T, V>(xr + c);
 #pragma unroll
       for (int k = 0; k < V; k++) s += to_f32(v.e[k]);
     }
+    if (V == 1 && row + gridDim.x < rows) fetch_ahead(xr + gridDim.x * ldx, cols);
     const float mu = wide_sum(s, red, half) * inv;
+#pragma unroll UNROLL
     for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
       const Vec<T, V> v = load_vec<T, V>(xr + c);
 #pragma unroll
@@ -508,54 +523,67 @@ __global__ void __launch_bounds__(WIDE)
       mean[row] = mu;
       rstd[row] = r;
     }
-    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
-      Vec<T, V> v = load_vec<T, V>(xr + c);
-      float w[V], b[V];
-      load_weights<V>(w, wb.w, wb.dtype, c, 1.0f);
-      load_weights<V>(b, wb.b, wb.dtype, c, 0.0f);
+    of_weights(wb.dtype, [&](auto type) {
+      typedef decltype(type) W;
+#pragma unroll UNROLL
+      for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+        Vec<T, V> v = load_vec<T, V>(xr + c);
+        float w[V], b[V];
+        load_weights<V, W>(w, wb.w, c, 1.0f);
+        load_weights<V, W>(b, wb.b, c, 0.0f);
 #pragma unroll
-      for (int k = 0; k < V; k++) v.e[k] = from_f32<T>(fmaf((to_f32(v.e[k]) - mu) * r, w[k], b[k]));
-      store_vec<T, V>(y + row * ldy + c, v);
-    }
+        for (int k = 0; k < V; k++) v.e[k] = from_f32<T>(fmaf((to_f32(v.e[k]) - mu) * r, w[k], b[k]));
+        store_vec<T, V>(y + row * ldy + c, v);
+      }
+    });
   }
 }
 
 // Their dx; the sums over rows are k_ln_cols's.
 template <typename T, int V>
-__global__ void __launch_bounds__(WIDE)
+__global__ void __launch_bounds__(WIDE, WIDE_PER_SM)
     k_ln_bwd_wide(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ x, int64_t ldx, int64_t rows, int cols,
                   Weights wb, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                   int64_t ldd) {
   __shared__ float red[2][1][32];
+  constexpr int UNROLL = V == 1 ? 8 : 2;
   int half = 0;
   const float inv = 1.0f / (float)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const float mu = mean[row], r = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
-      const Vec<T, V> xv = load_vec<T, V>(x + row * ldx + c), gv = load_vec<T, V>(dy + row * ldg + c);
-      float w[V];
-      load_weights<V>(w, wb.w, wb.dtype, c, 1.0f);
+    of_weights(wb.dtype, [&](auto type) {
+      typedef decltype(type) W;
+#pragma unroll UNROLL
+      for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+        const Vec<T, V> xv = load_vec<T, V>(x + row * ldx + c), gv = load_vec<T, V>(dy + row * ldg + c);
+        float w[V];
+        load_weights<V, W>(w, wb.w, c, 1.0f);
 #pragma unroll
-      for (int k = 0; k < V; k++) {
-        const float xh = (to_f32(xv.e[k]) - mu) * r, g = to_f32(gv.e[k]) * w[k];
-        s1 += g;
-        s2 = fmaf(g, xh, s2);
+        for (int k = 0; k < V; k++) {
+          const float xh = (to_f32(xv.e[k]) - mu) * r, g = to_f32(gv.e[k]) * w[k];
+          s1 += g;
+          s2 = fmaf(g, xh, s2);
+        }
       }
-    }
+    });
     const float m1 = wide_sum(s1, red, half) * inv, m2 = wide_sum(s2, red, half) * inv;
-    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
-      const Vec<T, V> xv = load_vec<T, V>(x + row * ldx + c), gv = load_vec<T, V>(dy + row * ldg + c);
-      Vec<T, V> o;
-      float w[V];
-      load_weights<V>(w, wb.w, wb.dtype, c, 1.0f);
+    of_weights(wb.dtype, [&](auto type) {
+      typedef decltype(type) W;
+#pragma unroll UNROLL
+      for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
+        const Vec<T, V> xv = load_vec<T, V>(x + row * ldx + c), gv = load_vec<T, V>(dy + row * ldg + c);
+        Vec<T, V> o;
+        float w[V];
+        load_weights<V, W>(w, wb.w, c, 1.0f);
 #pragma unroll
-      for (int k = 0; k < V; k++) {
-        const float xh = (to_f32(xv.e[k]) - mu) * r, g = to_f32(gv.e[k]) * w[k];
-        o.e[k] = from_f32<T>(r * (g - m1 - xh * m2));
+        for (int k = 0; k < V; k++) {
+          const float xh = (to_f32(xv.e[k]) - mu) * r, g = to_f32(gv.e[k]) * w[k];
+          o.e[k] = from_f32<T>(r * (g - m1 - xh * m2));
+        }
+        store_vec<T, V>(dx + row * ldd + c, o);
       }
-      store_vec<T, V>(dx + row * ldd + c, o);
-    }
+    });
   }
 }
 
@@ -572,7 +600,7 @@ __global__ void __launch_bounds__(COLS)
   float aw[V], ab[V];
 #pragma unroll
   for (int k = 0; k < V; k++) aw[k] = ab[k] = 0.0f;
-#pragma unroll 4
+#pragma unroll (V == 1 ? 8 : 4)
   for (int64_t row = first; row < end; row++) {
     const Vec<T, V> xv = load_vec_nc<T, V>(x + row * ldx + c), gv = load_vec_nc<T, V>(dy + row * ldg + c);
     const float mu = mean[row], r = rstd[row];
@@ -619,13 +647,14 @@ struct Plan {
   int v, e, lanes, threads;
 };
 
-inline Plan plan_for(int cols, int v) {
+// `most`: values of a row that its threads' registers may take.
+inline Plan plan_for(int cols, int v, int most) {
   Plan p = {v, MOST, 1, BLOCK};
   if (v <= 2) {
     p.e = cols <= 16 ? 4 : cols <= 8 * MAX_LANES ? 8 : MOST;
   }
   while (p.lanes < 32 && p.lanes * p.e < cols) p.lanes <<= 1;
-  if (p.lanes * p.e < cols) p.lanes = cols > p.e * MAX_LANES ? 0 : (cols + 32 * p.e - 1) / (32 * p.e) * 32;
+  if (p.lanes * p.e < cols) p.lanes = cols > most ? 0 : (cols + 32 * p.e - 1) / (32 * p.e) * 32;
   p.threads = p.lanes > 32 ? p.lanes : p.lanes ? BLOCK : WIDE;
   return p;
 }
@@ -658,9 +687,19 @@ int room_for(K kernel, size_t bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess ? F16_OK : F16_ERR_CUDA;
 }
 
+// Most values of a row in registers; beyond them the wide kernels.  Backward a row has 512 threads (of 128 registers
+// each); of 16 values in 2-byte loads some spill, so such rows end at 8 a thread (20,000 x 5,001 bf16 492 us, wide
+// 230 + 147; fp32 364, wide 229 + 176).  Forward it may have 768 (of 80 registers; 8,000 x 12,288 bf16 69 us, wide 132;
+// 3,000 x 12,001 bf16 55, 68), but not where a load is one fp32 value (13,000 x 9,001 227 us, wide 203).
+template <typename T, bool BACK>
+constexpr int most_of(int v) {
+  if (BACK) return (sizeof(T) == 2 && v == 1 ? 8 : MOST) * MAX_LANES;
+  return MOST * (sizeof(T) == 4 && v == 1 ? MAX_LANES : FWD_LANES);
+}
+
 // f(V, E, LANES) for a plan, as integral constants.
 template <int N> using Int = std::integral_constant<int, N>;
-template <typename T, typename F>
+template <typename T, bool BACK, typename F>
 void with_plan(const Plan& p, F f) {
   constexpr int VW = 16 / sizeof(T);
   const auto of_warp = [&](auto v, auto e) { p.lanes == 32 ? f(v, e, Int<32>()) : f(v, e, Int<0>()); };
@@ -674,7 +713,7 @@ void with_plan(const Plan& p, F f) {
   } else {
     if (p.e == 4) of_warp(Int<1>(), Int<4>());
     else if (p.e == 8) of_any(Int<1>(), Int<8>());
-    else f(Int<1>(), Int<MOST>(), Int<ROW_BLOCK>());
+    else if constexpr (most_of<T, BACK>(1) > 8 * MAX_LANES) f(Int<1>(), Int<MOST>(), Int<ROW_BLOCK>());
   }
 }
 
@@ -690,7 +729,8 @@ int forward(const T* x, int64_t rows, int cols, int64_t ldx, Weights wb, float e
             float* rstd, cudaStream_t st) {
   const void* ptrs[2] = {x, y};
   const int64_t lds[2] = {ldx, ldy};
-  const Plan p = plan_for(cols, vec_for(cols, sizeof(T), ptrs, lds, 2));
+  const int v = vec_for(cols, sizeof(T), ptrs, lds, 2);
+  const Plan p = plan_for(cols, v, most_of<T, false>(v));
   if (!p.lanes) {
     const int64_t grid = rows < WIDE_PER_SM * sm_count() ? rows : WIDE_PER_SM * sm_count();
     with_loads<T>(p, [&](auto v) {
@@ -700,7 +740,7 @@ int forward(const T* x, int64_t rows, int cols, int64_t ldx, Weights wb, float e
   }
   const unsigned grid = (unsigned)grid_rows(rows, p, FWD_WARPS);
   int rc = F16_OK;
-  with_plan<T>(p, [&](auto v, auto e, auto lanes) {
+  with_plan<T, false>(p, [&](auto v, auto e, auto lanes) {
     const auto k = k_ln_fwd<T, v(), e(), lanes()>;
     const size_t smem = Ring<T, v(), e(), 1>::bytes(p.threads);
     rc = room_for(k, smem);
@@ -715,7 +755,8 @@ int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, in
              cudaStream_t st) {
   const void* ptrs[3] = {dy, x, dx};
   const int64_t lds[3] = {ldg, ldx, ldd};
-  const Plan p = plan_for(cols, vec_for(cols, sizeof(T), ptrs, lds, 3));
+  const int v = vec_for(cols, sizeof(T), ptrs, lds, 3);
+  const Plan p = plan_for(cols, v, most_of<T, true>(v));
   const int64_t room = part ? part_floats / (2 * (int64_t)cols) : 0;
   int64_t grid = p.lanes ? grid_rows(rows, p, BWD_WARPS) : 0;
   int rc = F16_OK;
@@ -733,7 +774,7 @@ int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, in
     });
   } else {
     if (part && grid > room) grid = room;
-    with_plan<T>(p, [&](auto v, auto e, auto lanes) {
+    with_plan<T, true>(p, [&](auto v, auto e, auto lanes) {
       const auto k = k_ln_bwd<T, v(), e(), lanes()>;
       const size_t ring = Ring<T, v(), e(), 2>::bytes(p.threads), sums = p.lanes <= 32 ? BLOCK / 32 * 2 * (size_t)cols * sizeof(float) : 0;
       const size_t smem = ring > sums ? ring : sums;

@@ -72,7 +72,7 @@ def run(x, w, b, dy, eps=1e-5):
 # widths: one value; under a warp; odd; two to a load; vector tails; a block a row; the most that
 # registers take and one above it; re-read rows
 @pytest.mark.parametrize("dim", [1, 2, 3, 8, 17, 31, 33, 64, 184, 214, 215, 384, 512, 513, 1000, 1024, 2050, 4096, 4097,
-                                 8192, 8193, 8200, 20001])
+                                 8192, 8193, 8200, 12288, 12289, 12296, 20001])
 @pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
                                           (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16)])
 @pytest.mark.parametrize("rows", [1, 37])
@@ -84,7 +84,7 @@ def test_against_fp64(cuda, rows, dim, dtype, wdtype):
         check(got, v, t, name)
 
 
-@pytest.mark.parametrize("rows,dim", [(4099, 184), (5000, 512), (4711, 7), (1500, 1536), (2000, 9000)])
+@pytest.mark.parametrize("rows,dim", [(4099, 184), (5000, 512), (4711, 7), (1500, 1536), (2000, 9000), (1700, 4097), (500, 16384)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_many_rows(cuda, rows, dim, dtype):
     x, w, b, dy = make(cuda, rows, dim, dtype, torch.float32, rows)
