@@ -72,7 +72,7 @@ def run(x, w, b, dy, eps=1e-5):
 # widths: one value; under a warp; odd; two to a load; vector tails; a block a row; the most that
 # registers take and one above it; re-read rows
 @pytest.mark.parametrize("dim", [1, 2, 3, 8, 17, 31, 33, 64, 184, 214, 215, 384, 512, 513, 1000, 1024, 2050, 4096, 4097,
-                                 8192, 8193, 8200, 12288, 12289, 12296, 20001])
+                                 8192, 8193, 8200, 12288, 12289, 12290, 12296, 20001])
 @pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
                                           (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16)])
 @pytest.mark.parametrize("rows", [1, 37])
