@@ -139,6 +139,10 @@ _SIGS = {
                            C.c_int),
     "f16_layer_norm_bwd": ([_P, _I64, _P, _I64, _I64, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _I64, _P, _P, _P,
                             _I64, _P], C.c_int),
+    "f16_layer_norm_fwd_rest": ([_P, _I64, C.c_int, _I64, C.c_int, _P, _P, C.c_int, C.c_double, _P, _I64, _P, _P, _P,
+                                 _P], C.c_int),
+    "f16_layer_norm_bwd_rest": ([_P, _I64, _P, _I64, _I64, C.c_int, C.c_int, _P, C.c_int, _P, _P, _P, _P, _I64, _P, _P,
+                                 _P, _I64, _P], C.c_int),
     "f16_layer_norm_scratch_floats": ([_I64, C.c_int], _I64),
     "f16_scan_saved_floats": ([_I64, _I64, _I64], _I64),
     "f16_scan_scratch_floats": ([_I64, _I64, _I64], _I64),

@@ -36,11 +36,11 @@ def _forward(x, rows, weight, bias, eps, stats):
         wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
         at = stats.data_ptr() if stats is not None else None
         with _lib.on_device(x):
-            _lib.check(_lib.load().f16_layer_norm_fwd(
+            _lib.check(_lib.load().f16_layer_norm_fwd_rest(
                 rows.data_ptr(), n, dim, _row_stride(rows), _lib.DTYPES[x.dtype],
                 weight.data_ptr() if weight is not None else None, bias.data_ptr() if bias is not None else None,
                 _lib.DTYPES[wdtype], eps, y.data_ptr(), dim, at, at + 4 * n if at is not None else None,
-                _lib.raw_stream(x)), "f16_layer_norm_fwd")
+                at + 8 * n if at is not None else None, _lib.raw_stream(x)), "f16_layer_norm_fwd")
     return y
 
 
@@ -48,7 +48,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows = _rows(x)
-        stats = x.new_empty(2, rows.shape[0], dtype=torch.float32)
+        stats = x.new_empty(3, rows.shape[0], dtype=torch.float32)      # mean, what its rounding left, 1 / deviation
         ctx.wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
         ctx.save_for_backward(rows, weight, stats)
         return _forward(x, rows, weight, bias, eps, stats)
@@ -72,9 +72,9 @@ class _LayerNorm(torch.autograd.Function):
             room = lib.f16_layer_norm_scratch_floats(n, dim) if need_w or need_b else 0
             scratch = x.new_empty(room, dtype=torch.float32) if room else None
             at = stats.data_ptr()
-            _lib.check(lib.f16_layer_norm_bwd(
+            _lib.check(lib.f16_layer_norm_bwd_rest(
                 dy.data_ptr(), _row_stride(dy), x.data_ptr(), _row_stride(x), n, dim, _lib.DTYPES[x.dtype],
-                weight.data_ptr() if weight is not None else None, _lib.DTYPES[ctx.wdtype], at, at + 4 * n,
+                weight.data_ptr() if weight is not None else None, _lib.DTYPES[ctx.wdtype], at, at + 4 * n, at + 8 * n,
                 dx.data_ptr() if need_x else None, dim, dw.data_ptr() if need_w else None,
                 db.data_ptr() if need_b else None, scratch.data_ptr() if room else None, room,
                 _lib.raw_stream(x)), "f16_layer_norm_bwd")

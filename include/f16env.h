@@ -540,6 +540,16 @@ int f16_layer_norm_bwd(const void* dy, int64_t ldg, const void* x, int64_t ldx, 
                        int64_t scratch_floats, f16_stream_t stream);
 int64_t f16_layer_norm_scratch_floats(int64_t rows, int cols);
 
+/* The two with the mean in two parts, mean + rest ([rows], NULL: as above): what the mean's rounding to fp32 leaves, up
+ * to 2^-25 of it, else stands in the backward pass's xh as that part of the mean over the spread. */
+int f16_layer_norm_fwd_rest(const void* x, int64_t rows, int cols, int64_t ldx, int dtype, const void* weight,
+                            const void* bias, int wdtype, double eps, void* y, int64_t ldy, float* mean,
+                            float* rest, float* rstd, f16_stream_t stream);
+int f16_layer_norm_bwd_rest(const void* dy, int64_t ldg, const void* x, int64_t ldx, int64_t rows, int cols,
+                            int dtype, const void* weight, int wdtype, const float* mean, const float* rest,
+                            const float* rstd, void* dx, int64_t ldd, void* dweight, void* dbias,
+                            float* scratch, int64_t scratch_floats, f16_stream_t stream);
+
 /* A gated linear recurrence over time, each of batch x dim channels by itself:
  *   gated 0: h_t = gate_t h_{t-1} + x_t;   gated 1: f = sigmoid(gate_t), h_t = f h_{t-1} + (1 - f) x_t,
  * from h_{-1} = h0.  A reset at (t, b) drops the state before (h_t = x_t, or (1 - f) x_t); steps from
