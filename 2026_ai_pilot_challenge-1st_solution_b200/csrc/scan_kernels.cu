@@ -27,9 +27,9 @@
 // leak: a coefficient that is NaN itself makes B NaN as well, so the two cannot be confused.
 //
 // Measured on a B200 whose copy makes 6.55 TB/s, with a cold L2 (gated bf16, us, and the share of that rate of the
-// bytes a pass has to move): time not cut, 64 steps x 16,384 x 128, forward 145 (88%), backward 260 (81%); cut,
-// 65,536 steps x 1 x 1,024, fold + starts + walk 56 + 6 + 66 (50%) and 55 + 7 + 112 (60%); single step, fp32,
-// 131,072 x 128, 50 (103%).  What the cut costs is the fold's second read; without it that case's 16 warps
+// bytes a pass has to move): time not cut, 64 steps x 16,384 x 128, forward 155 (83%), backward 279 (75%); cut,
+// 65,536 steps x 1 x 1,024, fold + starts + walk 61 + 6 + 72 (44%) and 60 + 7 + 121 (55%); single step, fp32,
+// 131,072 x 128, 52 (99%).  What the cut costs is the fold's second read; without it that case's 16 warps
 // would walk through 65,536 steps alone.
 #include "typed.cuh"
 
@@ -85,29 +85,53 @@ __device__ __forceinline__ Vec<T, V> narrow(typename Lanes<V>::type f) {
 // f = sigmoid(g) and k = 1 - f: with e = exp(g), k = 1 / (1 + e), and f = e k where g is at most zero.  Above,
 // f is 1 - k, whose only error of its own is one rounding: e k of an open gate (g above 17, where f rounds to 1) often
 // is 1 - 2^-24, an error that is the same at every step of a steady gate and adds up over a sequence (0.4% of the
-// state over 65,536 steps).  exp(g) is held at 2^126 and below, where k is 2^-126.
-__device__ __forceinline__ float capped_exp2(float t) {
+// state over 65,536 steps).
+// e is 2^t, t = g / ln 2 rounded once: an error of up to |t| / 2 units of t's last place, which a small f or k would
+// show (63 half steps at a gate of 80).  So what t is off by, g - t ln 2 with ln 2 in two parts (Cody and Waite's
+// reduction), multiplies e by 1 + itself.  f and k are good to 12 half steps (2^-24) of themselves, 2^t (2^-22) and
+// the reciprocal (2^-23) being most of it; below 2^-126 they are zero.  It costs three product-sums for a pair: 64 x
+// 16,384 x 128 bf16 155 + 279 us, 150 + 287 with t alone and the gates worked out twice in the backward pass.
+// Gates are held at 88 to either side, where e is 0 or k is 0 (an infinite t has no remainder).
+__device__ __forceinline__ float capped(float g) {
+  float c;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, 0f42B00000;" : "=f"(c) : "f"(g));
+  return c;
+}
+__device__ __forceinline__ float exp2_of(float t) {
   float e;
-  asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(e) : "f"(t));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
   return e;
 }
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f, LN2_LOW = -1.9046542e-9f;     // ln 2 = LN2 + LN2_LOW
 __device__ __forceinline__ float reciprocal(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void sigmoid(float g, float& f, float& k) {
-  const float e = capped_exp2(g * 1.4426950408889634f);
+// k, and f as e k whatever the gate is.
+__device__ __forceinline__ void sigmoid_closed(float g, float& f, float& k) {
+  g = capped(g);
+  const float t = g * LOG2E, rest = fmaf(t, -LN2_LOW, fmaf(t, -LN2, g)), e0 = exp2_of(t), e = fmaf(e0, rest, e0);
   k = reciprocal(1.0f + e);
-  f = g > 0.0f ? 1.0f - k : e * k;
+  f = e * k;
 }
-__device__ __forceinline__ void sigmoid(Two g, Two& f, Two& k) {
-  const float2 t = split(g * two(1.4426950408889634f));
-  const Two e = two(capped_exp2(t.x), capped_exp2(t.y));
+__device__ __forceinline__ void sigmoid_closed(Two g, Two& f, Two& k) {
+  const float2 at = split(g);
+  g = two(capped(at.x), capped(at.y));
+  const Two t = g * two(LOG2E), rest = fma2(t, two(-LN2_LOW), fma2(t, two(-LN2), g));
+  const float2 ts = split(t);
+  const Two e0 = two(exp2_of(ts.x), exp2_of(ts.y)), e = fma2(e0, rest, e0);
   const float2 d = split(e + two(1.0f));
   k = two(reciprocal(d.x), reciprocal(d.y));
-  const float2 at = split(g), closed = split(e * k), open = split(fma2(k, two(-1.0f), two(1.0f)));
+  f = e * k;
+}
+__device__ __forceinline__ void sigmoid(float g, float& f, float& k) {
+  sigmoid_closed(g, f, k);
+  f = g > 0.0f ? 1.0f - k : f;
+}
+__device__ __forceinline__ void sigmoid(Two g, Two& f, Two& k) {
+  sigmoid_closed(g, f, k);
+  const float2 at = split(g), closed = split(f), open = split(fma2(k, two(-1.0f), two(1.0f)));
   f = two(at.x > 0.0f ? open.x : closed.x, at.y > 0.0f ? open.y : closed.y);
 }
 
@@ -443,6 +467,29 @@ template <typename T, int V> struct Inputs<T, V, true> {
   __device__ __forceinline__ typename Lanes<V>::type dh(int stage, int i) const {
     return with_dh ? widen(get(stage, 2, i)) : all_of<typename Lanes<V>::type>(0.0f);
   }
+  // A gate's f and 1 - f from the first pass over the chunk to the second, in place of its gate and x: of one
+  // channel both, of two the smaller one, with the sign set where that is f.
+  static constexpr bool KEEPS = true;
+  __device__ __forceinline__ void keep(int stage, int i, float g, float f, float k) const {
+    *at(stage, 0, i) = __float_as_uint(g > 0.0f ? 1.0f - k : f);
+    *at(stage, 1, i) = __float_as_uint(k);
+  }
+  __device__ __forceinline__ void keep(int stage, int i, Two g, Two f, Two k) const {
+    const float2 of = split(g), a = split(f), b = split(k);
+    *at(stage, 0, i) = __float_as_uint(of.x > 0.0f ? b.x : -a.x);
+    *at(stage, 1, i) = __float_as_uint(of.y > 0.0f ? b.y : -a.y);
+  }
+  __device__ __forceinline__ void kept(int stage, int i, float& f, float& k) const {
+    f = __uint_as_float(*at(stage, 0, i));
+    k = __uint_as_float(*at(stage, 1, i));
+  }
+  __device__ __forceinline__ void kept(int stage, int i, Two& f, Two& k) const {
+    const float x = __uint_as_float(*at(stage, 0, i)), y = __uint_as_float(*at(stage, 1, i));
+    const float bx = 1.0f - fabsf(x), by = 1.0f - fabsf(y);
+    const bool ox = __float_as_int(x) >= 0, oy = __float_as_int(y) >= 0;
+    f = two(ox ? bx : -x, oy ? by : -y);
+    k = two(ox ? x : bx, oy ? y : by);
+  }
   // Every lane its own 4 bytes.
   __device__ __forceinline__ void copy(int stage, int which, Line<T> from, int n) {
     unsigned to = (unsigned)__cvta_generic_to_shared(at(stage, which, 0));
@@ -487,6 +534,7 @@ template <typename T, int V> struct Inputs<T, V, true> {
 };
 template <typename T, int V> struct Inputs<T, V, false> {
   typedef int Buffer;
+  static constexpr bool KEEPS = false;
   Vec<T, V> in[3][CHUNK];
   bool with_dh;
   __device__ __forceinline__ Inputs(Buffer&, const Args& p, const Lane&) : with_dh(p.dh) {}
@@ -515,14 +563,21 @@ __device__ __forceinline__ void walk_back(const I& in, int stage, unsigned cut, 
   for (int i = 0; i < CHUNK; i++) {
     if (!PLAIN && i >= left) break;
     P a, b, k;
-    const P xf = widen(in.x(stage, i));
-    step_of<GATED>(widen(in.gate(stage, i)), xf, a, b, k);
+    const P xf = widen(in.x(stage, i)), g = widen(in.gate(stage, i));
+    if constexpr (GATED && I::KEEPS) {
+      sigmoid_closed(g, a, k);         // only for the chunk's own states: over 16 steps f's bias is 2^-20 at most
+      b = k * xf;
+      in.keep(stage, i, g, a, k);
+    } else {
+      step_of<GATED>(g, xf, a, b, k);
+    }
     const bool r = !PLAIN && (cut >> i & 1);
     const P hp = PLAIN ? h : pick(r, zero, h);
     d[i] = GATED ? a * less(hp, xf) : hp;
     h = PLAIN ? fma2(a, hp, b) : pick(r, b, fma2(a, hp, b));
   }
-  asm volatile("" ::: "memory");        // the gates are read and worked out again, not kept
+  // where they are not kept in shared memory the gates are read and worked out again: registers do not hold them
+  asm volatile("" ::: "memory");
   // what reaches a step's state from the step after it is pass * carry
   P pass = all_of<P>(1.0f);
   const int last = !PLAIN && left < CHUNK ? left - 1 : CHUNK - 1;
@@ -532,7 +587,8 @@ __device__ __forceinline__ void walk_back(const I& in, int stage, unsigned cut, 
   for (int i = CHUNK - 1; i >= 0; i--) {
     if (!PLAIN && i >= left) continue;
     P a, b, k;
-    step_of<GATED>(widen(in.gate(stage, i)), zero, a, b, k);
+    if constexpr (GATED && I::KEEPS) in.kept(stage, i, a, k);
+    else step_of<GATED>(widen(in.gate(stage, i)), zero, a, b, k);
     const P G = fma2(pass, carry, in.dh(stage, i));
     P ox = GATED ? G * k : G, og = ox * d[i];
     if (PLAIN) {
