@@ -9,6 +9,7 @@ import ctypes as C
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libf16env.so"
@@ -210,6 +211,14 @@ def on_device(t):
 def raw_stream(t):
     """stream_of as an integer, without the Python objects on the way (a microsecond of a small call)."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def transformed():
+    """A forward-mode level, a functorch transform or a trace is open: calls have to go through autograd.Function,
+    which records or refuses them, also where no gradient follows.  (A dual tensor needs no requires_grad, and a
+    trace would hold the empty output alone.)"""
+    return (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+            or torch._C._functorch.peek_interpreter_stack() is not None)
 
 
 def checked(t, dtypes, shape, label, like=None):

@@ -4,7 +4,8 @@
 tensors: fp32, bf16 or fp16 input, weight and bias in fp32 or the input's type (either may be
 None), statistics and sums in fp32, one rounding when a value is stored.  Backward gives the
 gradients of x, weight and bias in two launches; the sums over rows behind the weight's and bias's
-are made in a fixed order, so the same inputs give the same bits.  ``LayerNorm`` is
+are made in a fixed order, so the same inputs give the same bits.  Forward-mode derivatives, double backward
+and functorch transforms are refused.  ``LayerNorm`` is
 ``torch.nn.LayerNorm`` over one axis with that forward (CPU tensors take torch's): a drop-in that
 keeps the parameter names, and that ``splitmm.run_tower`` takes between its layers.
 
@@ -30,7 +31,7 @@ def _row_stride(x):
 
 
 def _forward(x, rows, weight, bias, eps, stats):
-    n, dim = rows.shape
+    n, dim = map(int, rows.shape)           # a trace has tensors there
     y = x.new_empty(x.shape)
     if n:
         wdtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
@@ -95,8 +96,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         bias = _lib.checked(bias, (torch.float32, x.dtype), shape, "layer_norm bias", x).contiguous()
         if weight is not None and weight.dtype != bias.dtype:
             raise TypeError("layer_norm weight and bias must have the same dtype")
-    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
-                                    or bias is not None and bias.requires_grad):
+    if _lib.transformed() or torch.is_grad_enabled() and (
+            x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _forward(x, _rows(x), weight, bias, float(eps), None)
 

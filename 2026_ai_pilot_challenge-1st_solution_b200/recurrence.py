@@ -8,6 +8,7 @@ rollout buffers are (a batch-first tensor goes in as ``t.transpose(0, 1)``, a vi
 drops the state before step t (``PPOTrainer.b_done`` as it is: the step begins a new episode),
 ``lengths[b]`` ends a padded sequence: later steps leave the state, return zeros and get zero gradients,
 and what they hold is not read.  The state is fp32 throughout; outputs have the inputs' type.
+Forward-mode derivatives, double backward and functorch transforms are refused.
 
 ``gated_step`` / ``linear_step`` are one step of it for a decision, the fp32 state updated in place.
 
@@ -48,12 +49,12 @@ def _at(t):
 
 def _scratch(lib, x):
     """(buffer, values in it) for the segments of a scan with few channels, or (None, 0)."""
-    n = lib.f16_scan_scratch_floats(*x.shape)
+    n = lib.f16_scan_scratch_floats(*map(int, x.shape))      # a trace has tensors there
     return (x.new_empty(n, dtype=torch.float32) if n else None), n
 
 
 def _args(gate, x, h0, reset, lengths, gated, h, hn, saved, scratch, dh=None, dhn=None, dgate=None, dx=None, dh0=None):
-    return _lib.ScanArgs(_lib.DTYPES[x.dtype], gated, *x.shape, *_place(gate), *_place(x), _at(h0), _at(reset),
+    return _lib.ScanArgs(_lib.DTYPES[x.dtype], gated, *map(int, x.shape), *_place(gate), *_place(x), _at(h0), _at(reset),
                          reset.element_size() if reset is not None else 0,
                          *(reset.stride() if reset is not None else (0, 0)), _at(lengths), *_place(h), _at(hn), _at(saved),
                          *_place(dh), _at(dhn), *_place(dgate), *_place(dx), _at(dh0),
@@ -62,7 +63,7 @@ def _args(gate, x, h0, reset, lengths, gated, h, hn, saved, scratch, dh=None, dh
 
 def _forward(gate, x, h0, reset, lengths, gated, keep):
     """(h, hn, the states that the backward pass needs if ``keep``); gate and x with unit stride along dim."""
-    steps, batch, dim = x.shape
+    steps, batch, dim = map(int, x.shape)
     h = _like(x)
     hn = x.new_empty(batch, dim, dtype=torch.float32)
     saved = None
@@ -124,7 +125,7 @@ def _scan(gate, x, h0, reset, lengths, gated, name):
         _lib.checked(reset, _FLAGS, x.shape[:2], "reset flags", x)
     if lengths is not None:
         lengths = _lib.checked(lengths, _I64, x.shape[1:2], "lengths", x).contiguous()
-    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or h0 is not None and h0.requires_grad):
+    if _lib.transformed() or torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or h0 is not None and h0.requires_grad):
         return _Scan.apply(gate, x, h0, reset, lengths, int(gated))
     return _forward(_strided(gate), _strided(x), h0, reset, lengths, int(gated), False)[:2]
 
