@@ -221,6 +221,14 @@ def transformed():
             or torch._C._functorch.peek_interpreter_stack() is not None)
 
 
+def refuse_transformed(name, *tensors):
+    """For calls that write their arguments in place and record nothing: no trace, no transform, no tangents."""
+    if transformed() and (torch._C._get_tracing_state() is not None
+                          or torch._C._functorch.peek_interpreter_stack() is not None
+                          or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
+        raise RuntimeError(f"{name} records nothing: it takes no part in traces, forward-mode or functorch transforms")
+
+
 def checked(t, dtypes, shape, label, like=None):
     """require_cuda_tensor for the calls whose time is the host's: t has one of ``dtypes``, ``shape`` (None:
     any) and the device of ``like`` (None: any)."""

@@ -161,6 +161,7 @@ def _step(gate, x, state, reset, out, gated, name):
         _lib.checked(out, (x.dtype,), shape, "output", x)
     if reset is not None:
         _lib.checked(reset, _FLAGS, shape[:1], "reset flags", x)
+    _lib.refuse_transformed(name, gate, x, state, out)
     batch, dim = shape
     if not batch or not dim:
         return out
@@ -183,7 +184,7 @@ def _step(gate, x, state, reset, out, gated, name):
 def gated_step(gate, x, state, reset=None, out=None):
     """One step of ``gated_scan`` for a decision: gate, x (batch, dim), state (batch, dim) fp32 updated in
     place, reset (batch,) flags or None.  Returns the new state in the inputs' type (``out``); no
-    gradient is recorded."""
+    gradient is recorded, traces and transforms are refused."""
     return _step(gate, x, state, reset, out, 1, "gated_step")
 
 
