@@ -870,6 +870,24 @@ int forward(const T* x, int64_t rows, int cols, int64_t ldx, Weights wb, float e
   return rc != F16_OK ? rc : launch_status();
 }
 
+// Slices of rows of k_ln_cols: four blocks an SM over all tiles of its columns.
+inline int64_t col_tiles(int cols, int v) { return (cols + (int64_t)COLS * v - 1) / (COLS * v); }
+inline int64_t col_slices(int64_t tiles) { return (4 * sm_count() + tiles - 1) / tiles; }
+
+// Most blocks that write column sums of rows this wide, whatever their alignment and number.
+template <typename T>
+int64_t sum_blocks(int cols) {
+  const int widths[3] = {16 / (int)sizeof(T), 2, 1};
+  int64_t most = 0;
+  for (int v : widths) {
+    if (cols % v) continue;
+    const Plan p = plan_for(cols, v, most_of<T, true>(v));
+    const int64_t n = p.lanes ? grid_rows(INT64_MAX / 2, p, BWD_WARPS) : col_slices(col_tiles(cols, v));
+    if (n > most) most = n;
+  }
+  return most;
+}
+
 template <typename T>
 int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, int cols, Weights wb,
              const Stats<const float>& stats, T* dx, int64_t ldd, float* part, int64_t part_floats, void* dw, void* db,
@@ -886,8 +904,8 @@ int backward(const T* dy, int64_t ldg, const T* x, int64_t ldx, int64_t rows, in
       const int64_t blocks = rows < WIDE_PER_SM * sm_count() ? rows : WIDE_PER_SM * sm_count();
       if (dx) k_ln_bwd_wide<T, v()><<<(unsigned)blocks, WIDE, 0, st>>>(dy, ldg, x, ldx, rows, cols, wb, stats, dx, ldd);
       if (part) {
-        const int64_t tiles = (cols + COLS * v() - 1) / (COLS * v());
-        grid = (4 * sm_count() + tiles - 1) / tiles;
+        const int64_t tiles = col_tiles(cols, v());
+        grid = col_slices(tiles);
         if (grid > rows) grid = rows;
         if (grid > room) grid = room;
         k_ln_cols<T, v()><<<dim3((unsigned)tiles, (unsigned)grid), COLS, 0, st>>>(dy, ldg, x, ldx, rows, cols, stats, part);
@@ -946,8 +964,7 @@ extern "C" int f16_layer_norm_fwd(const void* x, int64_t rows, int cols, int64_t
 
 extern "C" int64_t f16_layer_norm_scratch_floats(int64_t rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  // no block has less than one row, no SM more backward blocks than its warps allow (two warps a block at least)
-  const int64_t most = (int64_t)sm_count() * (ln::BWD_WARPS / 2);
+  const int64_t a = ln::sum_blocks<float>(cols), b = ln::sum_blocks<__half>(cols), most = a > b ? a : b;
   return 2 * (int64_t)cols * (rows < most ? rows : most);
 }
 
