@@ -146,7 +146,7 @@ class PPOConfig:
     # within 1e-3 of the fp32 networks at the same tensor rate as "bf16" (about 4e-3)
     policy_operand: str = "fp16"
     # "adam": torch.optim.Adam after clip_grad_norm_, as the reference; "adamw": optim.AdamW, the clip
-    # inside its step, with `weight_decay` and moments of `state_bits` (32 or 8)
+    # inside its step, with `weight_decay` and moments of `state_bits` (32 or 8), which "adam" refuses
     optimizer: str = "adam"
     weight_decay: float = 0.0
     state_bits: int = 32
@@ -155,6 +155,8 @@ class PPOConfig:
 def make_optimizer(params, lr, cfg):
     """The optimiser of a parameter list that ``cfg.optimizer`` names (eps 1e-5, ppo_gpu.py:1300)."""
     if cfg.optimizer == "adam":
+        if cfg.weight_decay != 0.0 or cfg.state_bits != 32:
+            raise ValueError("weight_decay and state_bits take optimizer='adamw'")
         return torch.optim.Adam(params, lr=lr, eps=1e-5)
     if cfg.optimizer == "adamw":
         return AdamW(params, lr=lr, eps=1e-5, weight_decay=cfg.weight_decay, state_bits=cfg.state_bits,
