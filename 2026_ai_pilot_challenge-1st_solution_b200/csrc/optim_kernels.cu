@@ -328,6 +328,17 @@ __device__ __forceinline__ void update_block(T* p, const T* g, int64_t n, int64_
     else store4(p, at + h * 128 + lane4, n, vec, pv[h]);
     if (MASTER) wp[32 * h] = *reinterpret_cast<const float4*>(ms[h]);
   }
+  if (!FULL && nu.clip != nu.clip) {              // what lies past the end is zero, not 0 times a NaN
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int i = h * 128 + lane4 + 2 * k;
+        const float2 a = split(m[h][k]), b = split(v[h][k]);
+        m[h][k] = two(at + i < n ? a.x : 0.0f, at + i + 1 < n ? a.y : 0.0f);
+        v[h][k] = two(at + i < n ? b.x : 0.0f, at + i + 1 < n ? b.y : 0.0f);
+      }
+  }
   if (BITS == 8) {
     unsigned m_most, v_most;
     bool finite;
