@@ -74,6 +74,15 @@ class _Bucket:
                 out[name] = flat[first:first + n].view(self.params[i].shape)
         return out
 
+    def clear_tails(self):
+        """Zero behind the tensors' ends: what a step expects there, and no tensor's state holds."""
+        for p, first in zip(self.params, self.firsts):
+            end = first + p.numel()
+            if end % BLOCK:
+                for name in ("exp_avg", "exp_avg_sq", "master"):
+                    if name in self.buffers:
+                        self.buffers[name][end:end + -end % BLOCK].zero_()
+
     def prepare(self, bits):
         """What every step's call has alike: the table of all tensors, and the flat buffers' addresses."""
         self.numels = [p.numel() for p in self.params]
@@ -206,6 +215,8 @@ class AdamW(torch.optim.Optimizer):
             new = state_dict["state"].get(k)
             for n, t in self.state[p].items():
                 t.zero_() if new is None else t.copy_(new[n])
+        for b in [b for bs in self._buckets for b in bs]:
+            b.clear_tails()
 
     def step(self, closure=None):
         """One step over every parameter with a gradient; returns the closure's loss, if any."""

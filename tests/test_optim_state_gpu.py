@@ -37,3 +37,23 @@ def test_tails_stay_zero_when_the_clip_is_nan(cuda, bits, dtype, value):
     assert torch.equal(p.isnan(), q.isnan())
     for name, tail in tails(opt, 700):
         assert bool((tail == 0).all()), name
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loaded_state_has_zero_tails(cuda, bits):
+    """Tails that something else filled are cleared by load_state_dict, the tensors' own values are the state's, and
+    an optimiser takes its own state back as it is."""
+    optim = pkg_module("optim")
+    p = torch.randn(700, device=cuda).bfloat16().requires_grad_()
+    p.grad = torch.randn(700, device=cuda).bfloat16()
+    opt = optim.AdamW([p], state_bits=bits)
+    opt.step()
+    keep = {n: t.clone() for n, t in opt.state[p].items()}
+    for name, flat in opt.state_buffers()[0].items():
+        if name in ("exp_avg", "exp_avg_sq", "master"):
+            flat[700:] = float("nan")
+    opt.load_state_dict(opt.state_dict())
+    for name, tail in tails(opt, 700):
+        assert bool((tail == 0).all()), name
+    for n, t in opt.state[p].items():
+        assert torch.equal(t.float(), keep[n].float()), n
