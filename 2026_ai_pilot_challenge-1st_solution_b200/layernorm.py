@@ -2,7 +2,8 @@
 
 ``layer_norm(x, weight, bias, eps)`` is ``torch.nn.functional.layer_norm`` over the last axis for CUDA
 tensors: fp32, bf16 or fp16 input, weight and bias in fp32 or the input's type (either may be
-None), statistics and sums in fp32, one rounding when a value is stored.  Backward gives the
+None), statistics and sums in fp32, one rounding when a value is stored.  Under ``torch.autocast`` 16-bit
+arguments are taken as fp32 and so is the output, as torch's.  Backward gives the
 gradients of x, weight and bias in two launches; the sums over rows behind the weight's and bias's
 are made in a fixed order, so the same inputs give the same bits.  Forward-mode derivatives, double backward
 and functorch transforms are refused.  ``LayerNorm`` is
@@ -17,6 +18,7 @@ from . import _lib
 
 
 _FLOATS = tuple(_lib.DTYPES)
+_HALVES = (torch.bfloat16, torch.float16)
 MAX_DIM = 2 ** 29
 
 
@@ -84,6 +86,8 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (module docstring)."""
+    if torch.is_autocast_enabled("cuda"):
+        x, weight, bias = (t.float() if torch.is_tensor(t) and t.dtype in _HALVES else t for t in (x, weight, bias))
     _lib.checked(x, _FLOATS, None, "layer_norm input")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
         raise ValueError("layer_norm needs a last axis of 1 to 2^29 values")
