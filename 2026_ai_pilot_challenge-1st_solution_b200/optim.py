@@ -176,11 +176,11 @@ class AdamW(torch.optim.Optimizer):
                 kinds.setdefault((p.dtype, p.device), []).append(p)
             if len({d for _, d in kinds} | {b.device for bs in self._buckets for b in bs}) > 1:
                 raise ValueError("AdamW parameters must lie on one device")
-        except Exception:
+            buckets = [_Bucket(ps, self.state_bits, self.master_weights and dtype != torch.float32)
+                       for (dtype, _), ps in kinds.items()]
+        except BaseException:
             self.param_groups.pop()
             raise
-        buckets = [_Bucket(ps, self.state_bits, self.master_weights and dtype != torch.float32)
-                   for (dtype, _), ps in kinds.items()]
         self._buckets.append(buckets)
         for b in buckets:
             for i, p in enumerate(b.params):
