@@ -148,6 +148,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_grad_norm, self.seed = max_grad_norm, int(seed) & (2 ** 64 - 1)
         self.grad_norm = None
         self._buckets = []          # one list of _Bucket for each group
+        self._members = []          # its tensors
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     @staticmethod
@@ -182,6 +183,7 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
         self._buckets.append(buckets)
+        self._members.append(list(group["params"]))
         for b in buckets:
             for i, p in enumerate(b.params):
                 self.state[p] = b.views(i)
@@ -225,8 +227,13 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         calls = []
-        for group, buckets in zip(self.param_groups, self._buckets):
+        if len(self.param_groups) != len(self._members):
+            raise RuntimeError("parameter groups are added with add_param_group, and not taken out")
+        for group, members, buckets in zip(self.param_groups, self._members, self._buckets):
             self._check_numbers(group)
+            params = group["params"]
+            if len(params) != len(members) or not all(map(operator.is_, params, members)):
+                raise RuntimeError("a group's parameters, or the groups' order, are not what they were when it was added")
             for b in buckets:
                 made = b.arguments()
                 if made is not None:
