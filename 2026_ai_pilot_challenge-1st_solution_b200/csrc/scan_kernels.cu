@@ -44,8 +44,11 @@ constexpr int MAX_SEGMENT = F16_SCAN_SEGMENT;      // most steps of a segment
 constexpr int64_t MAX_STEPS = 0x7fffffff - 2 * CHUNK;     // time indexes are 32-bit
 // Time is cut where the channels give fewer than ENOUGH_PER_SM warps an SM, into so many segments that there
 // are WARPS_PER_SM, but no more than MAX_CUTS (k_scan_starts takes so many at once) while they are not too long.
-// (Fold of 65,536 x 1 x 1,024 with 16 / 24 / 32 / 48 / 64 warps: 108, 91, 107, 90, 88 us when these were chosen.)
-constexpr int ENOUGH_PER_SM = 12, WARPS_PER_SM = 64, MAX_CUTS = 1024;
+// Forward + backward, us, gated bf16, with 4 / 6 / 8 / 10 warps an SM: 1,024 steps cut 198 / 283 / 365 / 450, not cut
+// 272 / 313 / 325 / 369; 4,096 steps cut 693 / 1,036 / 1,358 / 1,671, not cut 1,046 / 1,200 / 1,252 / 1,454.
+// With segments for 16 / 32 / 48 / 64 / 96 / 128 warps an SM: 65,536 x 1 x 1,024 bf16 339 / 344 / 337 / 326 / 330 / 327,
+// 512 x 64 x 512 bf16 109 / 103 / 100 / 101 / 101 / 107, 4,096 x 16 x 128 fp32 80 / 85 / 85 / 82 / 83 / 85.
+constexpr int ENOUGH_PER_SM = 7, WARPS_PER_SM = 64, MAX_CUTS = 1024;
 static_assert(CHUNK == 16, "the resets of a chunk are half a word");
 
 typedef f16_scan_args Args;
