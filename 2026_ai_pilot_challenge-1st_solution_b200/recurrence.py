@@ -10,6 +10,10 @@ drops the state before step t (``PPOTrainer.b_done`` as it is: the step begins a
 and what they hold is not read.  The state is fp32 throughout; outputs have the inputs' type.
 Forward-mode derivatives, double backward and functorch transforms are refused.
 
+A state that becomes infinite or NaN stays one of the two until a reset, as does an infinite gradient until the
+reset before it; which of the two can depend on how the call is cut into segments (where coefficients
+multiply to 0 before they meet an infinite state).
+
 ``gated_step`` / ``linear_step`` are one step of it for a decision, the fp32 state updated in place.
 
 ``rollout.gae`` is the recurrence of this kind that the framework had (in reverse time, with scalar
@@ -144,7 +148,9 @@ def gated_scan(gate, x, h0=None, reset=None, lengths=None):
 
 def linear_scan(a, x, h0=None, reset=None, lengths=None):
     """(h, hn) of h_t = a_t h_{t-1} + x_t; arguments as in ``gated_scan``.  Meant for coefficients of
-    size up to 1; the product of 8,192 successive ones has to stay in fp32's range."""
+    size up to 1.  Where larger ones are among them, the product of any up to 8,192 successive ones has to stay
+    in fp32's normal range: a call with few channels multiplies them before they meet the state, where one
+    with many does not."""
     return _scan(a, x, h0, reset, lengths, False, "linear_scan")
 
 

@@ -562,7 +562,8 @@ int f16_layer_norm_bwd_rest(const void* dy, int64_t ldg, const void* x, int64_t 
  * dh and dhn (one of them may be NULL: zero) and writes dgate, dx and dh0, each NULL where not
  * wanted.  scratch: f16_scan_scratch_floats values, 8-byte aligned (none of them are kept); with less or
  * NULL, time is not cut into segments, which is slow for few channels and many steps.  Coefficients
- * above 1 in size: the product of any 16 F16_SCAN_SEGMENT successive ones has to stay in fp32's range.
+ * above 1 in size: the product of any up to 16 F16_SCAN_SEGMENT successive ones has to stay in fp32's normal range.
+ * A state that is infinite or NaN stays one of the two until a reset; which one may depend on the cut.
  * steps below 2^31 - 32. */
 #define F16_SCAN_CHUNK 16
 #define F16_SCAN_SEGMENT 512
