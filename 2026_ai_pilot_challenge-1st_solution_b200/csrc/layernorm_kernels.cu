@@ -12,12 +12,13 @@
 //  * 16-bit rows: where the mean lies far above the spread all values are of one binade or two, and 2^13 fp16 or 2^16
 //    bf16 ones of a binade add up exactly in fp32 (a block's last addition keeps its error, the wide kernel adds
 //    its warps' sums in fp64), so the remainder of the division is all there is to know: no second sum.
-// `lanes` threads share a row -- a power of two, the fewest whose registers hold it -- so narrow
-// rows share a warp and wide rows take a block.  Blocks are persistent: weights stay in registers
+// `lanes` threads share a row -- a power of two up to a warp, whole warps beyond, the fewest whose registers
+// hold it -- so narrow rows share a warp and wide rows take a block.  Blocks are persistent: weights stay in registers
 // over all rows of a block, the next row is loaded while the current one is reduced, and in the
 // backward pass so do the columns' partial sums of dw and db, which leave the block once, to be
 // added up by k_ln_wgrad in a fixed order (no atomics: the same inputs give the same gradients).
-// Sums, statistics and partial sums are fp32; values are rounded once, when stored.
+// Sums, statistics and partial sums are fp32 (a thread's sum over its rows is one chain of additions: 221 of
+// them at 524,288 x 512); values are rounded once, when stored.
 //
 // Rows of a warp or less: sums of products are made of products rounded by themselves (pairs of values are multiplied by adding a
 // zero that the assembler does not know to be one; it would fuse the product with the sum after it): what
@@ -34,8 +35,8 @@ namespace ln {
 constexpr int BLOCK = 256;          // threads of a block whose rows take a warp or less
 constexpr int MAX_LANES = 512, FWD_LANES = 768;      // threads of a row, at most: see most_of
 // Most values of a row in one thread.  16-byte loads take so many; with narrower ones a thread takes 8, of rows
-// up to 16 values 4 (500,000 x 33 fp16, forward + backward: 8 a thread 100 us, 4 142 us, 2 188 us;
-// 300,000 x 15 bf16: 30, 25 and 36 us), and 16 again where 8 do not suffice.
+// up to 16 values 4 (500,000 x 33 fp16, forward + backward: 8 a thread 107 us, 4 149 us;
+// 300,000 x 15 bf16: 29 and 28 us), and 16 again where 8 do not suffice.
 constexpr int MOST = 16;
 constexpr int MAX_COLS = 1 << 29;   // column indexes are 32-bit
 constexpr int WIDE = 512, WIDE_PER_SM = 3;      // threads of a block on a row too wide for registers, blocks on an SM
@@ -190,7 +191,7 @@ struct Part {
 
 // The thread's parts of its next rows, N tensors' of each: on their way into shared memory two rows ahead
 // (one row a block in flight leaves HBM idle half of the time; 16,384 x 4,096 bf16, forward + backward: 2 / 3 / 4
-// slots 52 + 81, 44 + 79, 45 + 79 us, and 80 + 106 from registers), or, where a load is narrower than the 4 bytes
+// slots 54 + 82, 47 + 80, 48 + 80 us, and 80 + 106 from registers before the mean had two parts), or, where a load is narrower than the 4 bytes
 // that can be copied so, one row ahead in registers.  A thread reads what it copied itself, so no barrier.
 constexpr int SLOTS = 3;
 template <typename T, int V, int E, int N>
@@ -331,7 +332,7 @@ __device__ __forceinline__ float sum_of(const Two (&s)[2]) {
 }
 
 // s + a b with the product rounded by itself; where a row takes a block nothing is left to cancel, and the fused
-// operation saves a tenth of the forward pass (16,384 x 4,096 bf16 44 us for 47, backward 79 for 80).
+// operation saves some time (16,384 x 4,096 bf16 47 us for 48, backward 80 for 82).
 template <int LANES>
 __device__ __forceinline__ Two plus_product(Two s, Two a, Two b, Two zero) {
   if constexpr (LANES == ROW_BLOCK) return fma2(a, b, s);
@@ -566,7 +567,7 @@ __device__ __forceinline__ double wide_sum64(float v, float (*red)[2][32], int& 
 }
 
 // The block's next row into L2, a line of 128 bytes a thread, while the present one's sums are made: forward with
-// narrow loads only (13,000 x 9,001 fp32 245 -> 204 us; with 16-byte loads, and backward with any, it lost).
+// narrow loads only (13,000 x 9,001 fp32 257 -> 214 us; with 16-byte loads, and backward with any, it lost).
 template <typename T>
 __device__ __forceinline__ void fetch_ahead(const T* row, int cols) {
   constexpr int LINE = 128 / (int)sizeof(T);
@@ -574,8 +575,9 @@ __device__ __forceinline__ void fetch_ahead(const T* row, int cols) {
 }
 
 // Rows too wide for a block's registers: a block a row, V values a load, read again for each of the passes
-// (the second and third hit L1 and L2), several loads under way a thread: 4,096 x 16,384 bf16 90 us forward, 92 + 52
-// + 10 backward with the sums over rows, where one read of everything would take 41 and 61.
+// (the second and third hit L1 and L2), several loads under way a thread: 4,096 x 16,384 bf16 92 us forward, 93 + 52
+// + 10 backward with the sums over rows, where one read of everything would take 41 and 61 (rows of up to some
+// 100 KB would fit shared memory; a kernel that holds them there was not built).
 template <typename T, int V>
 __global__ void __launch_bounds__(WIDE, WIDE_PER_SM)
     k_ln_fwd_wide(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps,
@@ -797,7 +799,7 @@ inline int64_t grid_rows(int64_t rows, const Plan& p, int warps_per_sm) {
 }
 
 // Persistent warps per SM, which the registers allow (80 and 128 a thread).  Forward with 16 / 24 / 32 of them:
-// 16,384 x 4,096 bf16 49 / 44 / 54 us, 100,003 x 215 fp16 37 / 31 / 41.
+// 16,384 x 4,096 bf16 52 / 47 / 60 us, 100,003 x 215 fp16 36 / 29 / 37.
 constexpr int FWD_WARPS = 24, BWD_WARPS = 16;
 
 // Dynamic shared memory above 48 KB has to be asked for (on every device; it costs the host under a microsecond).
@@ -808,9 +810,9 @@ int room_for(K kernel, size_t bytes) {
 }
 
 // Most values of a row in registers; beyond them the wide kernels.  Backward a row has 512 threads (of 128 registers
-// each); of 16 values in 2-byte loads some spill, so such rows end at 8 a thread (20,000 x 5,001 bf16 492 us, wide
-// 230 + 147; fp32 364, wide 229 + 176).  Forward it may have 768 (of 80 registers; 8,000 x 12,288 bf16 69 us, wide 132;
-// 3,000 x 12,001 bf16 55, 68), but not where a load is one fp32 value (13,000 x 9,001 227 us, wide 203).
+// each); of 16 values in 2-byte loads some spill, so such rows end at 8 a thread (20,000 x 5,001 bf16 511 us, wide
+// 234 + 135; fp32 383, wide 266 + 149).  Forward it may have 768 (of 80 registers; 8,000 x 12,288 bf16 73 us, wide 137;
+// 3,000 x 12,001 bf16 57, 71), but not where a load is one fp32 value (13,000 x 9,001 250 us, wide 214).
 template <typename T, bool BACK>
 constexpr int most_of(int v) {
   if (BACK) return (sizeof(T) == 2 && v == 1 ? 8 : MOST) * MAX_LANES;
@@ -837,7 +839,7 @@ void with_plan(const Plan& p, F f) {
   }
 }
 
-// g(V) for rows too wide for registers (4,000 x 9,002 fp16 backward 66 + 39 us by two values a load, 78 + 58 by one).
+// g(V) for rows too wide for registers (4,000 x 9,002 fp16 backward 67 + 34 us by two values a load).
 template <typename T, typename G>
 void with_loads(const Plan& p, G g) {
   if (p.v == 16 / (int)sizeof(T)) g(Int<16 / (int)sizeof(T)>());

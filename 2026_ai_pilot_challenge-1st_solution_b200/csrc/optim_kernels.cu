@@ -7,8 +7,8 @@
 // Bound by HBM: a step reads p, g, m, v and writes p, m, v once, and the norm reads g once more.  The
 // tensors come as a table in the kernel's parameters (no device table to build or keep), their
 // moments lie in flat buffers that begin a new block of QBLOCK values with every tensor.  Persistent
-// blocks walk over pieces of PIECE values.  The norm is summed in fp64 over the blocks' partial sums,
-// each block in the same order; the step counts live on the device and the last block to finish
+// blocks walk over pieces of PIECE values.  The norm's squares are added 32 at a time in fp32, then in fp64, each
+// block in the same order; the step counts live on the device and the last block to finish
 // raises them, so a captured step counts when it is replayed.
 //
 // 8-bit moments: m as e4m3 and v as e5m2 in units of a fp32 scale for each QBLOCK values (the largest
@@ -22,9 +22,10 @@
 // 16-bit parameters may have fp32 master copies; a master counts while it rounds to its parameter,
 // else the parameter was set from outside and is taken instead.
 //
-// Measured on a B200 whose copy makes 6.55 TB/s (norm + update, us): 252 million fp32 parameters with 8-bit moments
-// 165 + 811 (93%, 76% of that rate), 300 tensors with 22 million bf16 parameters, fp32 moments and masters 14 + 123,
-// 1.3 million fp32 parameters 2.5 + 8.2.  The 8-bit update is bound by the instructions of its roundings (integer
+// Measured on a B200 whose copy makes 6.55 TB/s (norm + update, us, with a cold L2): 252 million fp32 parameters with
+// 8-bit moments 167 + 814 (92%, 76% of that rate), 300 tensors with 22 million bf16 parameters, fp32 moments and masters
+// 14 + 120, 1.3 million fp32 parameters 4 + 10; 252 million bf16 parameters with 8-bit moments 95 + 808, with masters 95 +
+// 933 (48% and 74%: the same instructions over fewer bytes).  The 8-bit update is bound by the instructions of its roundings (integer
 // pipe 60%, 2.7 of 4 issue slots), not by HBM; pairs of values in one instruction brought it from 956 to 847.
 #include <cuda_fp8.h>
 #include "typed.cuh"
@@ -164,8 +165,8 @@ __global__ void __launch_bounds__(THREADS)
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// x / s rounded towards zero (x >= 0, inv = 1 / s): a Newton step gives the nearest quotient, the sign of its
-// residual says whether that lies above the true one.  What the rounding to a code below looks at are whole
+// x / s rounded towards zero (x >= 0, inv = 1 / s): a Newton step with a fused residual (Markstein's method) gives
+// the nearest quotient, the sign of its residual says whether that lies above the true one.  What the rounding to a code below looks at are whole
 // units of the quotient's last place, so it decides as the exact quotient would; the nearest one would
 // fall on the wrong side of a code's border once in some 10^6 -- and often where a block's values all
 // shrink alike, which makes the quotients codes again and again.

@@ -435,7 +435,9 @@ __global__ void __launch_bounds__(START_THREADS)
 
 // A chunk of the backward pass's three inputs, as the lane's own values: in shared memory, where the copies of
 // the next chunk land while this one is worked on (4-byte lanes), or in registers.  Backward of 64 x 16,384 x 128
-// bf16: copies of 16 bytes 252 us, of each lane's own 4 bytes 305, chunks in registers 321 to 402.
+// bf16: copies of 16 bytes 280 us, of each lane's own 4 bytes 338, chunks in registers 412; the gates worked out twice in
+// place of kept 301.  Values of 2 bytes at odd widths or addresses are loaded into registers: 64 x 16,384 x 127, no
+// resets, 199 + 330, of 128 channels 146 + 247.
 constexpr int STAGES = 2;
 template <typename T, int V, bool STAGED> struct Inputs;
 template <typename T, int V> struct Inputs<T, V, true> {

@@ -3,12 +3,13 @@
 ``layer_norm(x, weight, bias, eps)`` is ``torch.nn.functional.layer_norm`` over the last axis for CUDA
 tensors: fp32, bf16 or fp16 input, weight and bias in fp32 or the input's type (either may be
 None), statistics and sums in fp32, one rounding when a value is stored.  Under ``torch.autocast`` 16-bit
-arguments are taken as fp32 and so is the output, as torch's.  Backward gives the
-gradients of x, weight and bias in two launches; the sums over rows behind the weight's and bias's
-are made in a fixed order, so the same inputs give the same bits.  Forward-mode derivatives, double backward
+arguments are taken as fp32 and so is the output, as torch's.  fp64 inputs are refused.  Backward gives the
+gradients of x, weight and bias in two launches (three for rows too wide for registers); the sums over rows
+behind the weight's and bias's are made in a fixed order, so the same inputs give the same bits.  Forward-mode derivatives, double backward
 and functorch transforms are refused.  ``LayerNorm`` is
-``torch.nn.LayerNorm`` over one axis with that forward (CPU tensors take torch's): a drop-in that
-keeps the parameter names, and that ``splitmm.run_tower`` takes between its layers.
+``torch.nn.LayerNorm`` over one axis with that forward (CPU tensors take torch's): it
+keeps the parameter names, and ``splitmm.run_tower`` takes it between its layers.  ``trainer.MLPActorCritic`` builds no
+towers with it, and ``policy.MlpWeights`` (the rollout's fused forward) refuses one.
 
 The reference normalises observations only (``rollout.RunningNorm``) and has no counterpart.
 """

@@ -1,4 +1,7 @@
-"""AdamW over many tensors in one launch, the gradients' clip included, moments in 32 or 8 bits.
+"""AdamW over many tensors a launch, the gradients' clip included, moments in 32 or 8 bits.
+
+A step is one launch for each group's parameters of one type (up to 720 tensors each), and one more of each for
+the gradients' norm where they are clipped.
 
 ``AdamW`` is ``torch.optim.AdamW`` (decoupled weight decay; with ``weight_decay=0`` torch.optim.Adam,
 the reference's optimiser, R/cuda_fdm/ppo_gpu.py:1300) for CUDA parameters, as a
@@ -18,6 +21,11 @@ the reference's optimiser, R/cuda_fdm/ppo_gpu.py:1300) for CUDA parameters, as a
 
 Moments, masters and step counts of a group's tensors of one type lie in flat buffers
 (``state_buffers``); ``state[p]`` holds the tensors' views of them.
+
+What torch's has and this one refuses: a tensor as ``lr``, a state of ``torch.optim.AdamW`` (its keys and step
+counts differ; ``load_state_dict`` takes this class's own form), copies and pickles of the optimiser,
+sparse gradients, parameters that are not contiguous or lie on several devices, groups changed other than by
+``add_param_group``.  ``amsgrad``, ``maximize``, ``foreach``, ``capturable`` and ``differentiable`` are not arguments.
 """
 import ctypes as C
 import operator

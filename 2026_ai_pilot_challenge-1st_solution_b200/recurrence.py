@@ -14,7 +14,8 @@ A state that becomes infinite or NaN stays one of the two until a reset, as does
 reset before it; which of the two can depend on how the call is cut into segments (where coefficients
 multiply to 0 before they meet an infinite state).
 
-``gated_step`` / ``linear_step`` are one step of it for a decision, the fp32 state updated in place.
+``gated_step`` / ``linear_step`` are one step of it for a decision, the fp32 state updated in place.  They are for
+a loop of the user's own: ``PPOTrainer``'s policies have no state, and ``ppo_update`` draws rows without regard to time.
 
 ``rollout.gae`` is the recurrence of this kind that the framework had (in reverse time, with scalar
 coefficients); the reference has no recurrent network left (its GRU was removed).
@@ -190,7 +191,8 @@ def _step(gate, x, state, reset, out, gated, name):
 def gated_step(gate, x, state, reset=None, out=None):
     """One step of ``gated_scan`` for a decision: gate, x (batch, dim), state (batch, dim) fp32 updated in
     place, reset (batch,) flags or None.  Returns the new state in the inputs' type (``out``); no
-    gradient is recorded, traces and transforms are refused."""
+    gradient is recorded, traces and transforms are refused.
+    ``out`` and ``state`` may be x's or gate's own memory, but share no part of it at another place."""
     return _step(gate, x, state, reset, out, 1, "gated_step")
 
 
