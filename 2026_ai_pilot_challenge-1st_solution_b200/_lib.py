@@ -213,20 +213,20 @@ def raw_stream(t):
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def transformed():
-    """A forward-mode level, a functorch transform or a trace is open: calls have to go through autograd.Function,
-    which records or refuses them, also where no gradient follows.  (A dual tensor needs no requires_grad, and a
-    trace would hold the empty output alone.)"""
-    return (forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
-            or torch._C._functorch.peek_interpreter_stack() is not None)
+def transformed(*tensors):
+    """A trace is open, or one of the tensors (or None) has a forward-mode tangent: the call has to go through
+    autograd.Function, which records or refuses it, also where no gradient follows.  (A dual tensor needs no
+    requires_grad, and a trace would hold the empty output alone.  Tensors inside functorch's transforms have no
+    address, which refuses them.)"""
+    return (torch._C._get_tracing_state() is not None
+            or forward_ad._current_level >= 0
+            and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors))
 
 
 def refuse_transformed(name, *tensors):
-    """For calls that write their arguments in place and record nothing: no trace, no transform, no tangents."""
-    if transformed() and (torch._C._get_tracing_state() is not None
-                          or torch._C._functorch.peek_interpreter_stack() is not None
-                          or any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
-        raise RuntimeError(f"{name} records nothing: it takes no part in traces, forward-mode or functorch transforms")
+    """For calls that write their arguments in place and record nothing."""
+    if transformed(*tensors):
+        raise RuntimeError(f"{name} records nothing: it takes no part in traces and forward-mode derivatives")
 
 
 def checked(t, dtypes, shape, label, like=None):

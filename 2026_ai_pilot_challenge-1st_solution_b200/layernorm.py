@@ -101,7 +101,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         bias = _lib.checked(bias, (torch.float32, x.dtype), shape, "layer_norm bias", x).contiguous()
         if weight is not None and weight.dtype != bias.dtype:
             raise TypeError("layer_norm weight and bias must have the same dtype")
-    if _lib.transformed() or torch.is_grad_enabled() and (
+    if _lib.transformed(x, weight, bias) or torch.is_grad_enabled() and (
             x.requires_grad or weight is not None and weight.requires_grad or bias is not None and bias.requires_grad):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _forward(x, _rows(x), weight, bias, float(eps), None)

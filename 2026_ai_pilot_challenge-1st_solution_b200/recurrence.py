@@ -130,7 +130,7 @@ def _scan(gate, x, h0, reset, lengths, gated, name):
         _lib.checked(reset, _FLAGS, x.shape[:2], "reset flags", x)
     if lengths is not None:
         lengths = _lib.checked(lengths, _I64, x.shape[1:2], "lengths", x).contiguous()
-    if _lib.transformed() or torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or h0 is not None and h0.requires_grad):
+    if _lib.transformed(gate, x, h0) or torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or h0 is not None and h0.requires_grad):
         return _Scan.apply(gate, x, h0, reset, lengths, int(gated))
     return _forward(_strided(gate), _strided(x), h0, reset, lengths, int(gated), False)[:2]
 
