@@ -311,7 +311,7 @@ __device__ __forceinline__ float mean_of(float total, float low, float n, float 
 template <bool EXACT>
 __device__ __forceinline__ float rstd_of(float squares, float delta, float n, float inv, float eps) {
   if (EXACT) return rsqrtf(fmaf(-delta, delta, squares * inv) + eps);
-  const float var = fmaf(-delta, delta, mean_of(squares, n, inv));
+  const float var = squares < __int_as_float(0x7f800000) ? fmaf(-delta, delta, mean_of(squares, n, inv)) : squares;
   return rsqrtf((var < 0.0f ? 0.0f : var) + eps);
 }
 __device__ __forceinline__ void store_stats(const Stats<float>& st, int64_t row, float mu, float delta, float r) {
