@@ -11,7 +11,7 @@
 //    beside their squares and taken out of them (16,384 x 4,096 forward 94 us, 91 without);
 //  * 16-bit rows: where the mean lies far above the spread all values are of one binade or two, and 2^13 fp16 or 2^16
 //    bf16 ones of a binade add up exactly in fp32 (a block's last addition keeps its error, the wide kernel adds
-//    its warps' sums in fp64), so the remainder of the division is all there is to know: no second sum.
+//    its threads' sums of CHAIN values in fp64), so the remainder of the division is all there is to know: no second sum.
 // `lanes` threads share a row -- a power of two up to a warp, whole warps beyond, the fewest whose registers
 // hold it -- so narrow rows share a warp and wide rows take a block.  Blocks are persistent: weights stay in registers
 // over all rows of a block, the next row is loaded while the current one is reduced, and in the
@@ -40,6 +40,7 @@ constexpr int MAX_LANES = 512, FWD_LANES = 768;      // threads of a row, at mos
 constexpr int MOST = 16;
 constexpr int MAX_COLS = 1 << 29;   // column indexes are 32-bit
 constexpr int WIDE = 512, WIDE_PER_SM = 3;      // threads of a block on a row too wide for registers, blocks on an SM
+constexpr int CHAIN = 256;          // values that a thread adds up in fp32 there
 
 // What a forward pass leaves for the backward one, a value a row each: the mean as mean + rest (rest may be NULL:
 // zero), and r.  Its rounding to one fp32 value, 2^-25 of the mean, would stand in xh as that part of the mean over
@@ -551,23 +552,20 @@ template <int N>
 __device__ __forceinline__ void wide_sums(float (&v)[2], float (*red)[2][32], int& half) {
   row_sums<ROW_BLOCK, N>(v, WIDE, red, half);
 }
-// The sum with its warps' sums added in fp64.
-__device__ __forceinline__ double wide_sum64(float v, float (*red)[2][32], int& half) {
-  float* r = red[half][0];
-  half ^= 1;
+__device__ __forceinline__ double wide_sum64(double v, double* red) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   const int lane = threadIdx.x & 31;
-  if (lane == 0) r[threadIdx.x >> 5] = v;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  double sum = lane < WIDE / 32 ? (double)r[lane] : 0.0;
+  v = lane < WIDE / 32 ? red[lane] : 0.0;
 #pragma unroll
-  for (int o = WIDE / 64; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  return __shfl_sync(~0u, sum, 0);
+  for (int o = WIDE / 64; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return __shfl_sync(~0u, v, 0);
 }
 
 // The block's next row into L2, a line of 128 bytes a thread, while the present one's sums are made: forward with
-// narrow loads only (13,000 x 9,001 fp32 257 -> 214 us; with 16-byte loads, and backward with any, it lost).
+// narrow loads only (13,000 x 9,001 fp32 257 -> 217 us; with 16-byte loads, and backward with any, it lost).
 template <typename T>
 __device__ __forceinline__ void fetch_ahead(const T* row, int cols) {
   constexpr int LINE = 128 / (int)sizeof(T);
@@ -575,7 +573,7 @@ __device__ __forceinline__ void fetch_ahead(const T* row, int cols) {
 }
 
 // Rows too wide for a block's registers: a block a row, V values a load, read again for each of the passes
-// (the second and third hit L1 and L2), several loads under way a thread: 4,096 x 16,384 bf16 92 us forward, 93 + 52
+// (the second and third hit L1 and L2), several loads under way a thread: 4,096 x 16,384 bf16 93 us forward, 92 + 52
 // + 10 backward with the sums over rows, where one read of everything would take 41 and 61 (rows of up to some
 // 100 KB would fit shared memory; a kernel that holds them there was not built).
 template <typename T, int V>
@@ -583,27 +581,35 @@ __global__ void __launch_bounds__(WIDE, WIDE_PER_SM)
     k_ln_fwd_wide(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols, Weights wb, float eps,
                   T* __restrict__ y, int64_t ldy, Stats<float> stats) {
   __shared__ float red[2][2][32];
+  __shared__ double red64[WIDE / 32];         // read before the row's next barrier, written after it
   constexpr int UNROLL = V * sizeof(T) <= 4 ? 8 : V == 2 ? 4 : 2;
   int half = 0;
   const float n = (float)cols, inv = 1.0f / n;
   [[maybe_unused]] const double inv64 = 1.0 / (double)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
-    float s[2] = {0.0f, 0.0f}, q[2] = {0.0f, 0.0f};
+    float s[2], q[2] = {0.0f, 0.0f};
+    double sum64 = 0.0;
+    for (int begin = 0; begin < cols; begin += WIDE * CHAIN) {
+      const int end = cols - begin < WIDE * CHAIN ? cols : begin + WIDE * CHAIN;
+      s[0] = 0.0f;
 #pragma unroll UNROLL
-    for (int c = threadIdx.x * V; c < cols; c += WIDE * V) {
-      const Vec<T, V> v = load_vec<T, V>(xr + c);
+      for (int c = begin + threadIdx.x * V; c < end; c += WIDE * V) {
+        const Vec<T, V> v = load_vec<T, V>(xr + c);
 #pragma unroll
-      for (int k = 0; k < V; k++) s[0] += to_f32(v.e[k]);
+        for (int k = 0; k < V; k++) s[0] += to_f32(v.e[k]);
+      }
+      sum64 += (double)s[0];
     }
     if (V <= 2 && row + gridDim.x < rows) fetch_ahead(xr + gridDim.x * ldx, cols);
     float mu, delta = 0.0f;
     if constexpr (EXACT_SUM<T>) {
-      const double total = wide_sum64(s[0], red, half), q = total * inv64;
+      const double total = wide_sum64(sum64, red64), q = total * inv64;
       const double mean = fma(fma(-q, (double)cols, total), inv64, q);          // as mean_of
       mu = (float)mean;
       delta = (float)(mean - (double)mu);
     } else {
+      s[0] = (float)sum64;
       wide_sums<1>(s, red, half);
       mu = mean_of(s[0], n, inv);
     }
@@ -812,7 +818,7 @@ int room_for(K kernel, size_t bytes) {
 // Most values of a row in registers; beyond them the wide kernels.  Backward a row has 512 threads (of 128 registers
 // each); of 16 values in 2-byte loads some spill, so such rows end at 8 a thread (20,000 x 5,001 bf16 511 us, wide
 // 234 + 135; fp32 383, wide 266 + 149).  Forward it may have 768 (of 80 registers; 8,000 x 12,288 bf16 73 us, wide 137;
-// 3,000 x 12,001 bf16 57, 71), but not where a load is one fp32 value (13,000 x 9,001 250 us, wide 214).
+// 3,000 x 12,001 bf16 57, 71), but not where a load is one fp32 value (13,000 x 9,001 250 us, wide 217).
 template <typename T, bool BACK>
 constexpr int most_of(int v) {
   if (BACK) return (sizeof(T) == 2 && v == 1 ? 8 : MOST) * MAX_LANES;
